@@ -467,6 +467,173 @@ int sa_paged_kv_append_lens(const void* k_new, const void* v_new,
                             const int64_t* vc_strides, int64_t bt_stride,
                             int dtype, sa_stream_t stream);
 
+/*
+ * RMS norm of each head's query and key rows and rotate-half RoPE, one pass
+ * over q [B, Hq, T, D] and k [B, Hkv, T, D] of dtype (SA_BF16, SA_F16,
+ * SA_F32).  For a row x with its head dim's weight w (nullable: ones):
+ *   z = w x / sqrt(mean(x^2) + eps),
+ *   y_d = z_d cos - z_{d+D/2} sin,  y_{d+D/2} = z_{d+D/2} cos + z_d sin
+ * in fp32, rounded once to dtype.  cos / sin: fp32 contiguous [n_pos, D/2];
+ * row (b, t) uses table row positions[b * pos_stride + t] (int32; NULL: row
+ * t), clamped to the table.  Weights: w_dtype SA_F32 or dtype.  D a multiple
+ * of 16 in 16..512; element strides (b, h, t, d) with unit d stride, the
+ * others multiples of 16 bytes; pointers 16-byte aligned; B * T <= 2^24.
+ * No counterpart in the reference.
+ */
+int sa_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, void* k_out,
+                        const void* q_weight, const void* k_weight,
+                        const float* cos_table, const float* sin_table,
+                        const int32_t* positions, int64_t pos_stride, int B,
+                        int Hq, int Hkv, int T, int D, int n_pos,
+                        const int64_t* q_strides, const int64_t* k_strides,
+                        const int64_t* qo_strides, const int64_t* ko_strides,
+                        float eps, int dtype, int w_dtype, sa_stream_t stream);
+
+/*
+ * Its backward: dq, dk (dtype) from dq_out, dk_out (dtype), and where given
+ * the weights' gradients dq_weight, dk_weight [D] (w_dtype), summed in fp32 in
+ * a fixed order.  workspace: sa_qk_norm_rope_bwd_workspace_size() bytes, 16-byte
+ * aligned, contents ignored; only read where a weight gradient is asked for.
+ * With no row (B * T or Hq + Hkv 0) nothing is written and asking for a weight
+ * gradient is refused.
+ */
+int64_t sa_qk_norm_rope_bwd_workspace_size(int B, int Hq, int Hkv, int T,
+                                           int D);
+int sa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out,
+                        const void* dk_out, void* dq, void* dk,
+                        void* dq_weight, void* dk_weight, const void* q_weight,
+                        const void* k_weight, const float* cos_table,
+                        const float* sin_table, const int32_t* positions,
+                        int64_t pos_stride, int B, int Hq, int Hkv, int T,
+                        int D, int n_pos, const int64_t* q_strides,
+                        const int64_t* k_strides, const int64_t* dqo_strides,
+                        const int64_t* dko_strides, const int64_t* dq_strides,
+                        const int64_t* dk_strides, float eps, int dtype,
+                        int w_dtype, float* workspace, int64_t workspace_bytes,
+                        sa_stream_t stream);
+
+/*
+ * The serving form, over packed tokens: q [n_tokens, Hq, D], k and v
+ * [n_tokens, Hkv, D] (element strides (token, h, d)); token i at position
+ * positions[i] (clamped to the tables).  Normed and rotated q goes to q_out;
+ * normed and rotated k, and v as it is, to row slots[i] % page_size of page
+ * slots[i] / page_size of the caches [n_pages, Hkv, page_size, D] (strides
+ * (page, h, row, d)), each value rounded once to cache_dtype (SA_F32, SA_F16,
+ * SA_BF16, SA_FP8_E4M3FN: to nearest, NaN past 464).  A token whose slot is
+ * negative or past the caches writes no k and v.  Slots of one call are
+ * distinct.  Types, head dims and alignment as sa_qk_norm_rope_fwd, cache rows
+ * of 16-byte multiples; n_pages * page_size < 2^31.
+ */
+int sa_paged_qk_norm_rope_append(
+    const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+    void* v_cache, const void* q_weight, const void* k_weight,
+    const float* cos_table, const float* sin_table, const int32_t* positions,
+    const int32_t* slots, int n_tokens, int Hq, int Hkv, int D, int n_pos,
+    int page_size, int n_pages, const int64_t* q_strides,
+    const int64_t* k_strides, const int64_t* v_strides,
+    const int64_t* qo_strides, const int64_t* kc_strides,
+    const int64_t* vc_strides, float eps, int dtype, int w_dtype,
+    int cache_dtype, sa_stream_t stream);
+
+/*
+ * Pages and maps of a serving step, from lengths on the device.  For sequence
+ * b (of B <= 4096) with context_lens[b] tokens and new_lens[b] to come (both
+ * taken as at least 0, the first as at most max_pages * page_size), the pages
+ * that its tokens need past those it has are popped off the stack free_pages[0
+ * .. n_free[0]) (n_pages entries of room) and entered into its row of
+ * block_table [B, max_pages].  Sequences are served in order; one that finds
+ * too few pages, or whose table or the n_tokens packed tokens end, is cut:
+ * lens_out[b] is the length that has pages.
+ *   starts [B + 1]: packed position of each sequence's first new token
+ *   slots, positions, sequences [n_tokens]: cache slot (page * page_size + row,
+ *     -1 for none), position and sequence (-1 past the last) of each token
+ *   n_free_out[0]: free pages left
+ * The outputs do not overlap the inputs; block_table is updated in place, only
+ * past the pages that a sequence has, so the same call again does the same.
+ * n_pages * page_size and max_pages * page_size < 2^31.
+ */
+int sa_paged_reserve(int32_t* block_table, const int32_t* context_lens,
+                     const int32_t* new_lens, const int32_t* free_pages,
+                     const int32_t* n_free, int32_t* slots, int32_t* positions,
+                     int32_t* sequences, int32_t* starts, int32_t* lens_out,
+                     int32_t* n_free_out, int B, int max_pages, int page_size,
+                     int n_pages, int n_tokens, int64_t bt_stride,
+                     sa_stream_t stream);
+
+/*
+ * The pages of the sequences whose finished[b] is not 0 go back on the stack,
+ * in the order of the sequences and their tables; their table entries become
+ * -1 (entries that name no page are skipped) and lens_out[b] 0, that of the
+ * others context_lens[b].  counts_ws: int32 [B] of workspace.  B >= 1.
+ */
+int sa_paged_release(int32_t* block_table, const int32_t* context_lens,
+                     const uint8_t* finished, int32_t* free_pages,
+                     const int32_t* n_free, int32_t* lens_out,
+                     int32_t* n_free_out, int32_t* counts_ws, int B,
+                     int max_pages, int page_size, int n_pages,
+                     int64_t bt_stride, sa_stream_t stream);
+
+/*
+ * bounds[page, h, 0, :] and [page, h, 1, :] (contiguous [n_pages, Hkv, 2, D] of
+ * the cache's type) = smallest and largest value of each key column over the
+ * page's tokens (NaN where one is), for the pages that hold tokens from_lens[b]
+ * .. to_lens[b] - 1 of each sequence; a page's tokens from its first on up to
+ * to_lens[b] count, also those before from_lens[b].  Table entries that name no
+ * page are skipped.  Page sizes, head dims (8..1024) and cache types as
+ * sa_paged_decode; max_pages * page_size < 2^30.
+ */
+int sa_paged_key_bounds(const void* k_cache, void* bounds,
+                        const int32_t* block_table, const int32_t* from_lens,
+                        const int32_t* to_lens, int B, int Hkv, int D,
+                        int page_size, int max_pages, int n_pages,
+                        const int64_t* kc_strides, int64_t bt_stride,
+                        int cache_dtype, sa_stream_t stream);
+
+/*
+ * Choice of pages for one query token of each sequence: pages [B, Hkv, top_k]
+ * (contiguous int32), table indexes in ascending order, then -1.  Of the
+ * np = ceil(context_lens[b] / page_size) pages of a sequence: all where np <=
+ * top_k, else the first n_first, the last n_last and those of the others with
+ * the largest
+ *   score = sum_d Q+_d bounds[page, h, 1, d] + Q-_d bounds[page, h, 0, d],
+ * Q+ / Q- = sum over the KV head's query heads of max(q, 0) / min(q, 0), in 64
+ * bits; equal scores: the lower page; NaN above all.  n_first + n_last <=
+ * top_k.  q [B, Hq, 1, D] of dtype SA_BF16 / SA_F16 / SA_F32 with unit d
+ * stride; bounds of cache_dtype (sa_paged_key_bounds).  workspace (8-byte
+ * aligned): sa_paged_select_workspace_size() bytes where top_k < max_pages.
+ */
+int64_t sa_paged_select_workspace_size(int B, int Hkv, int max_pages);
+int sa_paged_select_pages(const void* q, const void* bounds,
+                          const int32_t* block_table,
+                          const int32_t* context_lens, int32_t* pages, int B,
+                          int Hq, int Hkv, int D, int page_size, int max_pages,
+                          int n_pages, int top_k, int n_first, int n_last,
+                          const int64_t* q_strides, int64_t bt_stride,
+                          int dtype, int cache_dtype, void* workspace,
+                          int64_t workspace_bytes, sa_stream_t stream);
+
+/*
+ * sa_paged_decode over listed pages only: pages [B, Hkv, n_listed] (contiguous
+ * int32) holds indexes into the sequence's table row, in any order; those
+ * outside [0, max_pages) are skipped, and of a page the tokens below
+ * context_lens[b] count, once for every time it is listed.  Everything else as
+ * sa_paged_decode; workspace: sa_paged_sparse_workspace_size() bytes, 16-byte
+ * aligned, contents ignored.
+ */
+int64_t sa_paged_sparse_workspace_size(int B, int Hq, int Hkv, int D,
+                                       int n_listed, int page_size);
+int sa_paged_sparse_decode(const void* q, const void* k_cache,
+                           const void* v_cache, void* out,
+                           const int32_t* block_table,
+                           const int32_t* context_lens, const int32_t* pages,
+                           int B, int Hq, int Hkv, int D, int page_size,
+                           int max_pages, int n_pages, int n_listed,
+                           const int64_t* q_strides, const int64_t* kv_strides,
+                           const int64_t* vv_strides, const int64_t* o_strides,
+                           int64_t bt_stride, float scale, int dtype,
+                           float* workspace, int64_t workspace_bytes,
+                           sa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

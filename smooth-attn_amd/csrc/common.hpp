@@ -28,6 +28,17 @@ __device__ __forceinline__ T from_f32(float x) { return static_cast<T>(x); }
 __device__ __forceinline__ float fast_sqrt(float x) { return __builtin_amdgcn_sqrtf(x); }
 __device__ __forceinline__ float fast_rsqrt(float x) { return __builtin_amdgcn_rsqf(x); }
 
+// The smaller and the larger of two values of one integer type.  (min and max of
+// two 64-bit types that are not the same go through double in device code.)
+template <typename T>
+__device__ __forceinline__ T smaller(T a, T b) {
+    return b < a ? b : a;
+}
+template <typename T>
+__device__ __forceinline__ T larger(T a, T b) {
+    return a < b ? b : a;
+}
+
 // Lane-to-lane moves inside a 16-lane DPP row.
 template <int CTRL>
 __device__ __forceinline__ float dpp_mov(float v) {

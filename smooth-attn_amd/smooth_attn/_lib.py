@@ -93,6 +93,32 @@ SIGNATURES = {
     "sa_paged_kv_append_lens": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                         c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _I64P, _I64P,
                                         _I64P, c_int64, c_int, c_void_p]),
+    "sa_qk_norm_rope_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, _I64P, _I64P, _I64P,
+                                    _I64P, c_float, c_int, c_int, c_void_p]),
+    "sa_qk_norm_rope_bwd_workspace_size": (c_int64, [c_int, c_int, c_int, c_int, c_int]),
+    "sa_qk_norm_rope_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
+                                    c_int, c_int, c_int, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, c_float, c_int,
+                                    c_int, c_void_p, c_int64, c_void_p]),
+    "sa_paged_qk_norm_rope_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                                             c_int, c_int, c_int, c_int, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P,
+                                             c_float, c_int, c_int, c_int, c_void_p]),
+    "sa_paged_reserve": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p]),
+    "sa_paged_release": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_int, c_int, c_int, c_int, c_int64, c_void_p]),
+    "sa_paged_key_bounds": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                    c_int, c_int, _I64P, c_int64, c_int, c_void_p]),
+    "sa_paged_select_workspace_size": (c_int64, [c_int, c_int, c_int]),
+    "sa_paged_select_pages": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                      c_int, c_int, c_int, c_int, c_int, c_int, _I64P, c_int64, c_int, c_int,
+                                      c_void_p, c_int64, c_void_p]),
+    "sa_paged_sparse_workspace_size": (c_int64, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "sa_paged_sparse_decode": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                       c_int, c_int, c_int, c_int, c_int, c_int, c_int, _I64P, _I64P, _I64P, _I64P,
+                                       c_int64, c_float, c_int, c_void_p, c_int64, c_void_p]),
 }
 
 _lock = threading.Lock()
