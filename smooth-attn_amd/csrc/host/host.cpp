@@ -26,12 +26,15 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/version.h>
 
 #include <cmath>
 #include <cstring>
+#include <memory>
+#include <optional>
 #include <stdexcept>
 #include <string>
 
@@ -56,6 +59,17 @@ struct Abi {
     decltype(&sa_paged_decode) paged_decode = nullptr;
     decltype(&sa_paged_decode_workspace_size) paged_decode_workspace_size = nullptr;
     decltype(&sa_paged_kv_append_lens) paged_kv_append_lens = nullptr;
+    decltype(&sa_qk_norm_rope_fwd) qk_norm_rope_fwd = nullptr;
+    decltype(&sa_qk_norm_rope_bwd) qk_norm_rope_bwd = nullptr;
+    decltype(&sa_qk_norm_rope_bwd_workspace_size) qk_norm_rope_bwd_workspace_size = nullptr;
+    decltype(&sa_paged_qk_norm_rope_append) paged_qk_norm_rope_append = nullptr;
+    decltype(&sa_paged_reserve) paged_reserve = nullptr;
+    decltype(&sa_paged_release) paged_release = nullptr;
+    decltype(&sa_paged_key_bounds) paged_key_bounds = nullptr;
+    decltype(&sa_paged_select_pages) paged_select_pages = nullptr;
+    decltype(&sa_paged_select_workspace_size) paged_select_workspace_size = nullptr;
+    decltype(&sa_paged_sparse_decode) paged_sparse_decode = nullptr;
+    decltype(&sa_paged_sparse_workspace_size) paged_sparse_workspace_size = nullptr;
 } abi;
 
 template <typename F>
@@ -81,7 +95,18 @@ PyObject* py_bind(PyObject*, PyObject* table) {
         !bind_one(table, "sa_flash_bwd_workspace_size", abi.flash_bwd_workspace_size) ||
         !bind_one(table, "sa_paged_decode", abi.paged_decode) ||
         !bind_one(table, "sa_paged_decode_workspace_size", abi.paged_decode_workspace_size) ||
-        !bind_one(table, "sa_paged_kv_append_lens", abi.paged_kv_append_lens))
+        !bind_one(table, "sa_paged_kv_append_lens", abi.paged_kv_append_lens) ||
+        !bind_one(table, "sa_qk_norm_rope_fwd", abi.qk_norm_rope_fwd) ||
+        !bind_one(table, "sa_qk_norm_rope_bwd", abi.qk_norm_rope_bwd) ||
+        !bind_one(table, "sa_qk_norm_rope_bwd_workspace_size", abi.qk_norm_rope_bwd_workspace_size) ||
+        !bind_one(table, "sa_paged_qk_norm_rope_append", abi.paged_qk_norm_rope_append) ||
+        !bind_one(table, "sa_paged_reserve", abi.paged_reserve) ||
+        !bind_one(table, "sa_paged_release", abi.paged_release) ||
+        !bind_one(table, "sa_paged_key_bounds", abi.paged_key_bounds) ||
+        !bind_one(table, "sa_paged_select_pages", abi.paged_select_pages) ||
+        !bind_one(table, "sa_paged_select_workspace_size", abi.paged_select_workspace_size) ||
+        !bind_one(table, "sa_paged_sparse_decode", abi.paged_sparse_decode) ||
+        !bind_one(table, "sa_paged_sparse_workspace_size", abi.paged_sparse_workspace_size))
         return nullptr;
     Py_RETURN_NONE;
 }
@@ -505,6 +530,448 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// RMS norm + RoPE of queries and keys.
+// ---------------------------------------------------------------------------
+// A tensor argument that may be None: false where it is neither None nor plain.
+bool plain_or_none(PyObject* o, const Tensor*& t) {
+    t = nullptr;
+    return o == Py_None || (t = plain(o)) != nullptr;
+}
+
+const void* ptr(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
+
+// Weights [D] of x's type or fp32, of one type.
+bool norm_weight_ok(const Tensor* w, const Tensor& x) {
+    return w == nullptr || (w->dim() == 1 && w->size(0) == x.size(-1) && w->is_contiguous() && aligned16(*w) &&
+                            w->device() == x.device() &&
+                            (w->scalar_type() == x.scalar_type() || w->scalar_type() == at::kFloat));
+}
+int norm_weight_code(const Tensor* qw, const Tensor* kw, const Tensor& x) {
+    const Tensor* w = qw ? qw : kw;
+    return code_of(w ? w->scalar_type() : x.scalar_type());
+}
+
+bool norm_common_ok(const Tensor& q, const Tensor* qw, const Tensor* kw, const Tensor& cos, const Tensor& sin) {
+    const int64_t D = q.size(-1);
+    if (!float_code(code_of(q.scalar_type())) || D % 16 != 0 || D < 16 || D > 512 || !norm_weight_ok(qw, q) ||
+        !norm_weight_ok(kw, q) || (qw && kw && qw->scalar_type() != kw->scalar_type()))
+        return false;
+    for (const Tensor* t : {&cos, &sin})
+        if (t->dim() != 2 || t->size(1) != D / 2 || t->size(0) != cos.size(0) || t->size(0) == 0 ||
+            t->size(0) > INT32_MAX || t->scalar_type() != at::kFloat || !t->is_contiguous() || !aligned16(*t) ||
+            t->device() != q.device() || t->requires_grad())
+            return false;
+    return true;
+}
+
+bool qk_norm_ok(const Tensor& q, const Tensor& k, const Tensor* qw, const Tensor* kw, const Tensor& cos,
+                const Tensor& sin, const Tensor* pos) {
+    if (q.dim() != 4 || k.dim() != 4 || q.numel() == 0 || k.numel() == 0 || k.size(0) != q.size(0) ||
+        k.size(2) != q.size(2) || k.size(3) != q.size(3) || k.scalar_type() != q.scalar_type() ||
+        k.device() != q.device() || !norm_common_ok(q, qw, kw, cos, sin) || !operand_ok(q) || !operand_ok(k))
+        return false;
+    const int64_t B = q.size(0), T = q.size(2);
+    if (B > (1 << 24) || T > (1 << 24) || B * T > (1 << 24) || q.size(1) > 16383 || k.size(1) > 16383) return false;
+    if (pos == nullptr) return cos.size(0) >= T;
+    return pos->scalar_type() == at::kInt && pos->is_contiguous() && pos->device() == q.device() &&
+           ((pos->dim() == 1 && pos->size(0) == T) || (pos->dim() == 2 && pos->size(0) == B && pos->size(1) == T));
+}
+
+// A dense tensor in x's order of dims, if that keeps D innermost (kernels.py's rule).
+Tensor output_like(const Tensor& x) {
+    Tensor y = at::empty_like(x);
+    return y.stride(-1) == 1 ? y : at::empty(x.sizes(), x.options());
+}
+
+const int32_t* positions_ptr(const Tensor* pos) { return pos ? pos->data_ptr<int32_t>() : nullptr; }
+int64_t positions_stride(const Tensor* pos) { return pos && pos->dim() == 2 ? pos->size(1) : 0; }
+
+void qk_norm_fwd(const Tensor& q, const Tensor& k, const Tensor* qw, const Tensor* kw, const Tensor& cos,
+                 const Tensor& sin, const Tensor* pos, double eps, Tensor& yq, Tensor& yk) {
+    yq = output_like(q);
+    yk = output_like(k);
+    const c10::DeviceGuard guard(q.device());
+    check(abi.qk_norm_rope_fwd(q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), ptr(qw), ptr(kw),
+                               cos.data_ptr<float>(), sin.data_ptr<float>(), positions_ptr(pos), positions_stride(pos),
+                               dim(q, 0), dim(q, 1), dim(k, 1), dim(q, 2), dim(q, 3), dim(cos, 0), strides(q),
+                               strides(k), strides(yq), strides(yk), static_cast<float>(eps),
+                               code_of(q.scalar_type()), norm_weight_code(qw, kw, q), stream_of(q)),
+          "sa_qk_norm_rope_fwd");
+}
+
+struct QKNorm : public torch::autograd::Function<QKNorm> {
+    using MaybeTensor = std::optional<Tensor>;
+    static const Tensor* get(const MaybeTensor& t) { return t.has_value() ? &*t : nullptr; }
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const MaybeTensor& qw,
+                                 const MaybeTensor& kw, const Tensor& cos, const Tensor& sin, const MaybeTensor& pos,
+                                 double eps) {
+        Tensor yq, yk;
+        qk_norm_fwd(q, k, get(qw), get(kw), cos, sin, get(pos), eps, yq, yk);
+        variable_list save{q, k, cos, sin};
+        for (const MaybeTensor* t : {&qw, &kw, &pos})
+            if (t->has_value()) save.push_back(**t);
+        ctx->save_for_backward(std::move(save));
+        ctx->saved_data["given"] = int64_t(qw.has_value()) | int64_t(kw.has_value()) << 1 | int64_t(pos.has_value()) << 2;
+        ctx->saved_data["eps"] = eps;
+        return {yq, yk};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const bool again = at::GradMode::is_enabled() && (grads[0].requires_grad() || grads[1].requires_grad());
+        const at::AutoGradMode off(false);
+        const variable_list saved = ctx->get_saved_variables();
+        const int64_t given = ctx->saved_data["given"].toInt();
+        const Tensor* opt[3] = {nullptr, nullptr, nullptr};  // q_weight, k_weight, positions
+        int at_saved = 4;
+        for (int i = 0; i < 3; ++i)
+            if (given >> i & 1) opt[i] = &saved[at_saved++];
+        const auto fix = [](const Tensor& t) { return operand_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous); };
+        // (unpack hooks may hand back other layouts, and other types or sizes, which are refused)
+        TORCH_CHECK_VALUE(saved[0].is_cuda() && saved[0].dim() == 4 && saved[1].dim() == 4 &&
+                              float_code(code_of(saved[0].scalar_type())),
+                          "the saved tensors of the norm must have the shapes and dtype that forward saved");
+        for (const Tensor* t : std::initializer_list<const Tensor*>{&saved[1], &saved[2], &saved[3], opt[0], opt[1],
+                                                                   opt[2], &grads[0], &grads[1]})
+            TORCH_CHECK_VALUE(t == nullptr || (t->is_cuda() && t->device() == saved[0].device()),
+                              "the norm's tensors must live on the same CUDA device as q");
+        const Tensor q = fix(saved[0]), k = fix(saved[1]);
+        const auto plain_table = [](const Tensor& t) {
+            return t.is_contiguous() && aligned16(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+        };
+        const Tensor cos = plain_table(saved[2]), sin = plain_table(saved[3]);
+        Tensor w[2], pos;
+        for (int i = 0; i < 2; ++i)
+            if (opt[i]) w[i] = plain_table(*opt[i]);
+        if (opt[2]) pos = opt[2]->contiguous();
+        const Tensor *qw = opt[0] ? &w[0] : nullptr, *kw = opt[1] ? &w[1] : nullptr, *ps = opt[2] ? &pos : nullptr;
+        TORCH_CHECK_VALUE(q.sizes() == grads[0].sizes() && k.sizes() == grads[1].sizes() &&
+                              qk_norm_ok(q, k, qw, kw, cos, sin, ps),
+                          "the saved tensors of the norm must have the shapes and dtype that forward saved");
+        const Tensor gq = fix(grads[0].to(q.scalar_type())), gk = fix(grads[1].to(q.scalar_type()));
+        const int B = dim(q, 0), Hq = dim(q, 1), Hkv = dim(k, 1), T = dim(q, 2), D = dim(q, 3);
+        Tensor dq = output_like(q), dk = output_like(k), dw[2], ws;
+        // (only the tensors given have an edge)
+        if (qw && ctx->needs_input_grad(2)) dw[0] = at::empty_like(*qw);
+        if (kw && ctx->needs_input_grad(qw ? 3 : 2)) dw[1] = at::empty_like(*kw);
+        const bool any = dw[0].defined() || dw[1].defined();
+        const int64_t ws_bytes = any ? abi.qk_norm_rope_bwd_workspace_size(B, Hq, Hkv, T, D) : 0;
+        if (any) ws = at::empty({ws_bytes / 4}, q.options().dtype(at::kFloat));
+        const auto out = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+        {
+            const c10::DeviceGuard guard(q.device());
+            check(abi.qk_norm_rope_bwd(
+                      q.data_ptr(), k.data_ptr(), gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), out(dw[0]),
+                      out(dw[1]), ptr(qw), ptr(kw), cos.data_ptr<float>(), sin.data_ptr<float>(), positions_ptr(ps),
+                      positions_stride(ps), B, Hq, Hkv, T, D, dim(cos, 0), strides(q), strides(k), strides(gq),
+                      strides(gk), strides(dq), strides(dk), static_cast<float>(ctx->saved_data["eps"].toDouble()),
+                      code_of(q.scalar_type()), norm_weight_code(qw, kw, q),
+                      any ? ws.data_ptr<float>() : nullptr, ws_bytes, stream_of(q)),
+                  "sa_qk_norm_rope_bwd");
+        }
+        variable_list result{dq, dk, dw[0], dw[1]};
+        if (again) {  // differentiated twice: the second time raises
+            const at::AutoGradMode on(true);
+            for (Tensor& t : result)
+                if (t.defined()) t.set_requires_grad(true);
+            auto error = std::make_shared<torch::autograd::DelayedError>(
+                "trying to differentiate twice a function that has one derivative (sp2norm_qk_norm_rope)",
+                static_cast<int64_t>(result.size()));
+            result = (*error)(std::move(result));
+        }
+        return {result[0], result[1], result[2], result[3], Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps) -> (q', k') or None.
+PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *q, *k, *qw, *kw, *cos, *sin, *pos;
+    double eps;
+    if (n != 8 || !plain_mode() || !(q = plain(a[0])) || !(k = plain(a[1])) || !plain_or_none(a[2], qw) ||
+        !plain_or_none(a[3], kw) || !(cos = plain(a[4])) || !(sin = plain(a[5])) || !plain_or_none(a[6], pos) ||
+        !as_double(a[7], eps) || !qk_norm_ok(*q, *k, qw, kw, *cos, *sin, pos))
+        Py_RETURN_NONE;
+    Tensor yq, yk;
+    {
+        const NoGil released;
+        const auto wants = [](const Tensor* t) { return t && t->requires_grad(); };
+        if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(qw) || wants(kw))) {
+            const auto maybe = [](const Tensor* t) { return t ? std::optional<Tensor>(*t) : std::nullopt; };
+            variable_list y = QKNorm::apply(*q, *k, maybe(qw), maybe(kw), *cos, *sin, maybe(pos), eps);
+            yq = y[0];
+            yk = y[1];
+        } else {
+            qk_norm_fwd(*q, *k, qw, kw, *cos, *sin, pos, eps, yq, yk);
+        }
+    }
+    PyObject* pair = PyTuple_New(2);
+    if (pair == nullptr) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(yq));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(yk));
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------------------
+// Serving operators.
+// ---------------------------------------------------------------------------
+// A block table [>= B, max_pages] of rows that do not overlap.
+bool table_ok(const Tensor& t, int64_t B, const Tensor& like) {
+    return t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) >= B && t.size(1) > 0 && t.size(1) <= INT32_MAX &&
+           t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) >= t.size(1)) && t.device() == like.device();
+}
+int64_t table_stride(const Tensor& t) { return std::max(t.stride(0), t.size(1)); }
+
+// A contiguous int32 vector of at least n entries.
+bool ints_ok(const Tensor& t, int64_t n, const Tensor& like) {
+    return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) >= n && t.is_contiguous() &&
+           t.device() == like.device();
+}
+
+// Caches [n_pages, Hkv, block_size, D] in the layout that the kernels take.
+bool cache_ok(const Tensor& c, int64_t Hkv, int block_size, int64_t D, const Tensor& like) {
+    return c.dim() == 4 && c.numel() > 0 && c.size(1) == Hkv && c.size(2) == block_size && c.size(3) == D &&
+           code_of(c.scalar_type()) >= 0 && c.size(0) <= INT32_MAX / block_size && D % (16 / c.element_size()) == 0 &&
+           c.device() == like.device() && operand_ok(c);
+}
+bool power_of_two(int x) { return x > 0 && (x & (x - 1)) == 0; }
+
+// paged_norm_append(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, eps,
+// block_size) -> q' or None.
+PyObject* py_paged_norm_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *q, *k, *v, *qw, *kw, *cos, *sin, *pos, *slots, *kc, *vc;
+    double eps;
+    int block_size;
+    if (n != 13 || !plain_mode() || !(q = plain(a[0])) || !(k = plain(a[1])) || !(v = plain(a[2])) ||
+        !plain_or_none(a[3], qw) || !plain_or_none(a[4], kw) || !(cos = plain(a[5])) || !(sin = plain(a[6])) ||
+        !(pos = plain(a[7])) || !(slots = plain(a[8])) || !(kc = plain(a[9])) || !(vc = plain(a[10])) ||
+        !as_double(a[11], eps) || !as_int(a[12], block_size) || block_size == 0)
+        Py_RETURN_NONE;
+    if (q->dim() != 3 || k->dim() != 3 || q->numel() == 0 || k->numel() == 0 || v->sizes() != k->sizes() ||
+        k->size(0) != q->size(0) || k->size(2) != q->size(2) || q->size(0) > (1 << 24) || q->size(1) > 16383 ||
+        k->size(1) > 16383 || !norm_common_ok(*q, qw, kw, *cos, *sin))
+        Py_RETURN_NONE;
+    for (const Tensor* t : {k, v})
+        if (t->scalar_type() != q->scalar_type() || t->device() != q->device()) Py_RETURN_NONE;
+    const int64_t N = q->size(0), Hkv = k->size(1), D = q->size(2);
+    if (!operand_ok(*q) || !operand_ok(*k) || !operand_ok(*v) || !ints_ok(*pos, N, *q) || !ints_ok(*slots, N, *q) ||
+        pos->size(0) != N || slots->size(0) != N || !cache_ok(*kc, Hkv, block_size, D, *q) ||
+        !cache_ok(*vc, Hkv, block_size, D, *q) || vc->sizes() != kc->sizes() || vc->scalar_type() != kc->scalar_type())
+        Py_RETURN_NONE;
+    Tensor out;
+    {
+        const NoGil released;
+        const at::AutoGradMode off(false);
+        out = output_like(*q);
+        const c10::DeviceGuard guard(q->device());
+        check(abi.paged_qk_norm_rope_append(
+                  q->data_ptr(), k->data_ptr(), v->data_ptr(), out.data_ptr(), kc->data_ptr(), vc->data_ptr(), ptr(qw),
+                  ptr(kw), cos->data_ptr<float>(), sin->data_ptr<float>(), pos->data_ptr<int32_t>(),
+                  slots->data_ptr<int32_t>(), static_cast<int>(N), dim(*q, 1), static_cast<int>(Hkv),
+                  static_cast<int>(D), dim(*cos, 0), block_size, dim(*kc, 0), strides(*q), strides(*k), strides(*v),
+                  strides(out), strides(*kc), strides(*vc), static_cast<float>(eps), code_of(q->scalar_type()),
+                  norm_weight_code(qw, kw, *q), code_of(kc->scalar_type()), stream_of(*q)),
+              "sa_paged_qk_norm_rope_append");
+    }
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// What reserve and release take as they are: a table of B rows, lengths [B],
+// the stack and its count.
+bool maps_ok(const Tensor& table, const Tensor& lens, const Tensor& free_pages, const Tensor& n_free, int block_size) {
+    if (table.dim() != 2 || table.numel() == 0 || block_size == 0) return false;
+    const int64_t B = table.size(0);
+    return B <= 4096 && table_ok(table, B, table) && ints_ok(lens, B, table) && lens.size(0) == B &&
+           ints_ok(free_pages, 1, table) && n_free.scalar_type() == at::kInt && n_free.numel() == 1 &&
+           n_free.device() == table.device() && std::max(free_pages.size(0), table.size(1)) <= INT32_MAX / block_size;
+}
+
+// paged_reserve(block_table, context_lens, new_lens, free_pages, n_free, n_tokens, block_size) -> (slots,
+// positions, sequences, starts, context_lens, n_free) or None.
+PyObject* py_paged_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *table, *lens, *fresh, *free_pages, *n_free;
+    int n_tokens, block_size;
+    if (n != 7 || !plain_mode() || !(table = plain(a[0])) || !(lens = plain(a[1])) || !(fresh = plain(a[2])) ||
+        !(free_pages = plain(a[3])) || !(n_free = plain(a[4])) || !as_int(a[5], n_tokens) || !as_int(a[6], block_size) ||
+        !maps_ok(*table, *lens, *free_pages, *n_free, block_size) || !ints_ok(*fresh, table->size(0), *table) ||
+        fresh->size(0) != table->size(0))
+        Py_RETURN_NONE;
+    Tensor out[6];
+    {
+        const NoGil released;
+        const int64_t B = table->size(0);
+        const int64_t sizes[6] = {n_tokens, n_tokens, n_tokens, B + 1, B, 1};
+        for (int i = 0; i < 6; ++i) out[i] = at::empty({sizes[i]}, table->options());
+        const c10::DeviceGuard guard(table->device());
+        const auto p = [](const Tensor& t) { return t.data_ptr<int32_t>(); };
+        check(abi.paged_reserve(p(*table), p(*lens), p(*fresh), p(*free_pages), p(*n_free), p(out[0]), p(out[1]),
+                                p(out[2]), p(out[3]), p(out[4]), p(out[5]), static_cast<int>(B), dim(*table, 1),
+                                block_size, dim(*free_pages, 0), n_tokens, table_stride(*table), stream_of(*table)),
+              "sa_paged_reserve");
+    }
+    PyObject* all = PyTuple_New(6);
+    if (all == nullptr) return nullptr;
+    for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(all, i, THPVariable_Wrap(out[i]));
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_release(block_table, context_lens, finished, free_pages, n_free, block_size) -> (context_lens, n_free) or None.
+PyObject* py_paged_release(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *table, *lens, *finished, *free_pages, *n_free;
+    int block_size;
+    if (n != 6 || !plain_mode() || !(table = plain(a[0])) || !(lens = plain(a[1])) || !(finished = plain(a[2])) ||
+        !(free_pages = plain(a[3])) || !(n_free = plain(a[4])) || !as_int(a[5], block_size) ||
+        !maps_ok(*table, *lens, *free_pages, *n_free, block_size) || finished->scalar_type() != at::kBool ||
+        finished->dim() != 1 || finished->size(0) != table->size(0) || !finished->is_contiguous() ||
+        finished->device() != table->device())
+        Py_RETURN_NONE;
+    Tensor out, left, counts;
+    {
+        const NoGil released;
+        const int64_t B = table->size(0);
+        out = at::empty({B}, table->options());
+        left = at::empty({1}, table->options());
+        counts = at::empty({B}, table->options());
+        const c10::DeviceGuard guard(table->device());
+        const auto p = [](const Tensor& t) { return t.data_ptr<int32_t>(); };
+        check(abi.paged_release(p(*table), p(*lens), static_cast<const uint8_t*>(finished->data_ptr()), p(*free_pages),
+                                p(*n_free), p(out), p(left), p(counts), static_cast<int>(B), dim(*table, 1), block_size,
+                                dim(*free_pages, 0), table_stride(*table), stream_of(*table)),
+              "sa_paged_release");
+    }
+    PyObject* pair = PyTuple_New(2);
+    if (pair == nullptr) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(out));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(left));
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
+// Bounds of a cache [n_pages, Hkv, block_size, D], contiguous [n_pages, Hkv, 2, D].
+bool bounds_ok(const Tensor& b, const Tensor& like) {
+    return b.dim() == 4 && b.numel() > 0 && b.size(2) == 2 && b.size(0) <= INT32_MAX && b.is_contiguous() &&
+           aligned16(b) && b.device() == like.device() && code_of(b.scalar_type()) >= 0 && b.size(3) <= 1024 &&
+           b.size(3) % 8 == 0 && (b.element_size() != 1 || b.size(3) % 16 == 0);
+}
+
+// paged_key_bounds(k_cache, block_table, from_lens, to_lens, bounds, block_size) -> bool: whether it ran.
+PyObject* py_paged_key_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *kc, *table, *from, *to, *bounds;
+    int block_size;
+    if (n != 6 || !plain_mode() || !(kc = plain(a[0])) || !(table = plain(a[1])) || !(from = plain(a[2])) ||
+        !(to = plain(a[3])) || !(bounds = plain(a[4])) || !as_int(a[5], block_size) || !power_of_two(block_size) ||
+        kc->dim() != 4 || table->dim() != 2)
+        Py_RETURN_FALSE;
+    const int64_t B = table->size(0), Hkv = kc->size(1), D = kc->size(3);
+    if (B == 0 || B > INT32_MAX || !cache_ok(*kc, Hkv, block_size, D, *kc) || !table_ok(*table, B, *kc) ||
+        !ints_ok(*from, B, *kc) || !ints_ok(*to, B, *kc) || !bounds_ok(*bounds, *kc) ||
+        bounds->scalar_type() != kc->scalar_type() || bounds->size(0) != kc->size(0) || bounds->size(1) != Hkv ||
+        bounds->size(3) != D)
+        Py_RETURN_FALSE;
+    {
+        const NoGil released;
+        const c10::DeviceGuard guard(kc->device());
+        check(abi.paged_key_bounds(kc->data_ptr(), bounds->data_ptr(), table->data_ptr<int32_t>(),
+                                   from->data_ptr<int32_t>(), to->data_ptr<int32_t>(), static_cast<int>(B),
+                                   static_cast<int>(Hkv), static_cast<int>(D), block_size, dim(*table, 1), dim(*kc, 0),
+                                   strides(*kc), table_stride(*table), code_of(kc->scalar_type()), stream_of(*kc)),
+              "sa_paged_key_bounds");
+    }
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// One query token of each sequence, [B, Hq, 1, D].
+bool decode_q_ok(const Tensor& q, int64_t Hkv) {
+    return q.dim() == 4 && q.size(2) == 1 && q.numel() > 0 && q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX &&
+           Hkv > 0 && q.size(1) % Hkv == 0 && operand_ok(q);
+}
+
+// paged_select_pages(q, bounds, block_table, context_lens, top_k, n_first, n_last, block_size) -> pages or None.
+PyObject* py_paged_select_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *q, *bounds, *table, *lens;
+    int top_k, n_first, n_last, block_size;
+    if (n != 8 || !plain_mode() || !(q = plain(a[0])) || !(bounds = plain(a[1])) || !(table = plain(a[2])) ||
+        !(lens = plain(a[3])) || !as_int(a[4], top_k) || !as_int(a[5], n_first) || !as_int(a[6], n_last) ||
+        !as_int(a[7], block_size) || !power_of_two(block_size) || top_k < 1 || top_k >= (1 << 24) ||
+        static_cast<int64_t>(n_first) + n_last > top_k)
+        Py_RETURN_NONE;
+    if (!bounds_ok(*bounds, *bounds) || !decode_q_ok(*q, bounds->size(1)) || !float_code(code_of(q->scalar_type())) ||
+        q->size(3) != bounds->size(3) || q->device() != bounds->device() || !table_ok(*table, q->size(0), *q) ||
+        !ints_ok(*lens, q->size(0), *q) || bounds->size(0) > INT32_MAX / block_size)
+        Py_RETURN_NONE;
+    Tensor pages;
+    {
+        const NoGil released;
+        const int B = dim(*q, 0), Hkv = dim(*bounds, 1), W = dim(*table, 1);
+        pages = at::empty({B, Hkv, top_k}, table->options());
+        const int64_t ws_bytes = top_k < W ? abi.paged_select_workspace_size(B, Hkv, W) : 0;
+        Tensor ws;
+        if (ws_bytes > 0) ws = at::empty({(ws_bytes + 7) / 8}, table->options().dtype(at::kDouble));
+        const c10::DeviceGuard guard(q->device());
+        check(abi.paged_select_pages(q->data_ptr(), bounds->data_ptr(), table->data_ptr<int32_t>(),
+                                     lens->data_ptr<int32_t>(), pages.data_ptr<int32_t>(), B, dim(*q, 1), Hkv,
+                                     dim(*q, 3), block_size, W, dim(*bounds, 0), top_k, n_first, n_last, strides(*q),
+                                     table_stride(*table), code_of(q->scalar_type()), code_of(bounds->scalar_type()),
+                                     ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, stream_of(*q)),
+              "sa_paged_select_pages");
+    }
+    return THPVariable_Wrap(pages);
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_sparse(q, k_cache, v_cache, block_table, context_lens, pages, scale or None, block_size) -> out or None.
+PyObject* py_paged_sparse(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *q, *k, *v, *table, *lens, *pages;
+    int block_size;
+    if (n != 8 || !plain_mode() || !(q = plain(a[0])) || !(k = plain(a[1])) || !(v = plain(a[2])) ||
+        !(table = plain(a[3])) || !(lens = plain(a[4])) || !(pages = plain(a[5])) || !as_int(a[7], block_size) ||
+        !power_of_two(block_size) || k->dim() != 4 || !decode_q_ok(*q, k->size(1)))
+        Py_RETURN_NONE;
+    const int64_t B = q->size(0), Hq = q->size(1), D = q->size(3), Hkv = k->size(1);
+    const int qc = code_of(q->scalar_type()), kc = code_of(k->scalar_type());
+    const bool mixed = qc == SA_BF16 && kc == SA_FP8_E4M3FN;  // (other pairs convert q first)
+    if (!(mixed || (qc == kc && float_code(qc))) || Hq / Hkv > 32 || D % (mixed ? 16 : 8) != 0 || D > 512 ||
+        !paging_ok(*q, B, Hkv, D, block_size, *k, *v, *table, *lens) || !table_ok(*table, B, *q) ||
+        !ints_ok(*lens, B, *q) || k->size(0) > INT32_MAX / block_size || pages->dim() != 3 || pages->size(0) != B ||
+        pages->size(1) != Hkv || pages->size(2) > INT32_MAX || pages->scalar_type() != at::kInt ||
+        !pages->is_contiguous() || pages->device() != q->device())
+        Py_RETURN_NONE;
+    double scale;
+    if (a[6] == Py_None)
+        scale = 1.0 / std::sqrt(static_cast<double>(D));
+    else if (!as_double(a[6], scale))
+        Py_RETURN_NONE;
+    Tensor out;
+    {
+        const NoGil released;
+        out = at::empty({B, Hq, D}, q->options().dtype(at::kBFloat16).requires_grad(false));
+        const int b = static_cast<int>(B), hq = static_cast<int>(Hq), d = static_cast<int>(D);
+        const int hkv = static_cast<int>(Hkv), listed = dim(*pages, 2);
+        const int64_t ws_bytes =
+            std::max<int64_t>(16, abi.paged_sparse_workspace_size(b, hq, hkv, d, listed, block_size));
+        Tensor ws = at::empty({(ws_bytes + 3) / 4}, out.options().dtype(at::kFloat));
+        const c10::DeviceGuard guard(q->device());
+        check(abi.paged_sparse_decode(q->data_ptr(), k->data_ptr(), v->data_ptr(), out.data_ptr(),
+                                      table->data_ptr<int32_t>(), lens->data_ptr<int32_t>(), pages->data_ptr<int32_t>(),
+                                      b, hq, hkv, d, block_size, dim(*table, 1), dim(*k, 0), listed, strides(*q),
+                                      strides(*k), strides(*v), strides(out), table_stride(*table),
+                                      static_cast<float>(scale), mixed ? SA_PAGED_DTYPES(qc, kc) : qc,
+                                      ws.data_ptr<float>(), ws.numel() * 4, stream_of(*q)),
+              "sa_paged_sparse_decode");
+    }
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 template <typename F>
 PyCFunction fast(F f) {
     return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
@@ -519,6 +986,22 @@ PyMethodDef methods[] = {
      "paged(q, k_cache, v_cache, block_table, context_lens, scale, block_size) -> out or None"},
     {"paged_append", fast(py_paged_append), METH_FASTCALL,
      "paged_append(k_cache, v_cache, k_new, v_new, block_table, context_lens, block_size) -> lens or None"},
+    {"qk_norm_rope", fast(py_qk_norm_rope), METH_FASTCALL,
+     "qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps) -> (q', k') or None"},
+    {"paged_norm_append", fast(py_paged_norm_append), METH_FASTCALL,
+     "paged_norm_append(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, eps, block_size) "
+     "-> q' or None"},
+    {"paged_reserve", fast(py_paged_reserve), METH_FASTCALL,
+     "paged_reserve(block_table, context_lens, new_lens, free_pages, n_free, n_tokens, block_size) -> 6 tensors or "
+     "None"},
+    {"paged_release", fast(py_paged_release), METH_FASTCALL,
+     "paged_release(block_table, context_lens, finished, free_pages, n_free, block_size) -> 2 tensors or None"},
+    {"paged_key_bounds", fast(py_paged_key_bounds), METH_FASTCALL,
+     "paged_key_bounds(k_cache, block_table, from_lens, to_lens, bounds, block_size) -> bool"},
+    {"paged_select_pages", fast(py_paged_select_pages), METH_FASTCALL,
+     "paged_select_pages(q, bounds, block_table, context_lens, top_k, n_first, n_last, block_size) -> pages or None"},
+    {"paged_sparse", fast(py_paged_sparse), METH_FASTCALL,
+     "paged_sparse(q, k_cache, v_cache, block_table, context_lens, pages, scale, block_size) -> out or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native call path (see csrc/host/host.cpp).", -1, methods,

@@ -509,8 +509,8 @@ extern "C" int sa_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, vo
     using namespace sa;
     const int chk = check_sizes(B, Hq, Hkv, T, D, n_pos, dtype, w_dtype);
     if (chk != 0) return chk > 0 ? 0 : chk;
-    if (!q || !k || !q_out || !k_out || !cos_table || !sin_table || !q_strides || !k_strides || !qo_strides ||
-        !ko_strides)
+    if ((Hq > 0 && (!q || !q_out)) || (Hkv > 0 && (!k || !k_out)) || !cos_table || !sin_table || !q_strides ||
+        !k_strides || !qo_strides || !ko_strides)
         return SA_ERR_NULL_POINTER;
     if (!strides16(q_strides, 4, dtype) || !strides16(k_strides, 4, dtype) || !strides16(qo_strides, 4, dtype) ||
         !strides16(ko_strides, 4, dtype) || !aligned16(q) || !aligned16(k) || !aligned16(q_out) || !aligned16(k_out) ||
@@ -560,8 +560,8 @@ extern "C" int sa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_
     const int chk = check_sizes(B, Hq, Hkv, T, D, n_pos, dtype, w_dtype);
     if (chk < 0) return chk;
     if (chk > 0) return dq_weight || dk_weight ? SA_ERR_UNSUPPORTED : 0;  // (no row: the caller clears dw)
-    if (!q || !k || !dq_out || !dk_out || !dq || !dk || !cos_table || !sin_table || !q_strides || !k_strides ||
-        !dqo_strides || !dko_strides || !dq_strides || !dk_strides)
+    if ((Hq > 0 && (!q || !dq_out || !dq)) || (Hkv > 0 && (!k || !dk_out || !dk)) || !cos_table || !sin_table ||
+        !q_strides || !k_strides || !dqo_strides || !dko_strides || !dq_strides || !dk_strides)
         return SA_ERR_NULL_POINTER;
     if (!strides16(q_strides, 4, dtype) || !strides16(k_strides, 4, dtype) || !strides16(dqo_strides, 4, dtype) ||
         !strides16(dko_strides, 4, dtype) || !strides16(dq_strides, 4, dtype) || !strides16(dk_strides, 4, dtype) ||
@@ -621,8 +621,9 @@ extern "C" int sa_paged_qk_norm_rope_append(const void* q, const void* k, const 
     if (chk != 0) return chk > 0 ? 0 : chk;
     if (page_size <= 0 || n_pages < 0 || static_cast<int64_t>(page_size) * n_pages > INT32_MAX) return SA_ERR_BAD_SHAPE;
     if (!float_type(cache_dtype) && cache_dtype != SA_FP8_E4M3FN) return SA_ERR_BAD_DTYPE;
-    if (!q || !k || !v || !q_out || !k_cache || !v_cache || !cos_table || !sin_table || !positions || !slots ||
-        !q_strides || !k_strides || !v_strides || !qo_strides || !kc_strides || !vc_strides)
+    // (a cache of no pages stores nothing)
+    if ((Hq > 0 && (!q || !q_out)) || (Hkv > 0 && (!k || !v || (n_pages > 0 && (!k_cache || !v_cache)))) || !cos_table ||
+        !sin_table || !positions || !slots || !q_strides || !k_strides || !v_strides || !qo_strides || !kc_strides || !vc_strides)
         return SA_ERR_NULL_POINTER;
     if (!strides16(q_strides, 3, dtype) || !strides16(k_strides, 3, dtype) || !strides16(v_strides, 3, dtype) ||
         !strides16(qo_strides, 3, dtype) || !strides16(kc_strides, 4, cache_dtype) ||

@@ -157,6 +157,8 @@ class NothingOrdinary:
         return None
 
     norm_out = causal_norm = flash = paged = paged_append = _none
+    qk_norm_rope = paged_norm_append = paged_reserve = paged_release = _none
+    paged_key_bounds = paged_select_pages = paged_sparse = _none
 
 
 def _load_host(lib):

@@ -7,7 +7,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernels import _DTYPE_CODE, _check_same_device, _device_of, _flash_operand, _rope_tables, _stream
+from .kernels import _DTYPE_CODE, _check_same_device, _device_of, _flash_operand, _native, _rope_tables, _stream
 
 
 __all__ = ["sp2norm_qk_norm_rope"]
@@ -160,6 +160,9 @@ def sp2norm_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, 
     ``z = x * rsqrt(mean(x^2) + eps) * weight``, then the pair (d, d + D/2) of z
     is turned by its angle; fp32 inside, rounded once.  Returns (q', k') for
     ``sp2norm_flash_attention``."""
+    y = _native().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)
+    if y is not None:
+        return y
     _check_tensors(q=q, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin, positions=positions)
     if q.ndim != 4 or k.ndim != 4:
         raise ValueError("q and k must be [B, H, T, D] tensors")

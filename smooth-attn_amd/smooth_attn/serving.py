@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .kernels import (_CACHE_CODE, _DTYPE_CODE, _PAGED_CACHE_DTYPES, _check_paging_args, _check_same_device,
-                      _device_of, _flash_operand, _paged_dtype_code, _rope_tables, _stream)
+                      _device_of, _flash_operand, _native, _paged_dtype_code, _rope_tables, _stream)
 from .qk_norm import _check_norm_args, _check_tensors, _int32, _norm_weights, _output_like
 
 __all__ = ["PagedReservation", "sp2norm_paged_key_bounds", "sp2norm_paged_qk_norm_rope_append",
@@ -87,6 +87,9 @@ def sp2norm_paged_reserve(block_table, context_lens, new_lens, free_pages, n_fre
     context_lens in the result says how many tokens have pages, and the others'
     slots are -1.  Returns a PagedReservation; only block_table changes, so
     pass its n_free and context_lens to the next call."""
+    out = _native().paged_reserve(block_table, context_lens, new_lens, free_pages, n_free, n_tokens, block_size)
+    if out is not None:
+        return PagedReservation._make(out)
     _check_tensors(block_table=block_table, context_lens=context_lens, new_lens=new_lens, free_pages=free_pages,
                    n_free=n_free)
     B, W = _check_maps(block_table, {"context_lens": context_lens, "new_lens": new_lens}, free_pages, n_free,
@@ -113,6 +116,9 @@ def sp2norm_paged_release(block_table, context_lens, finished, free_pages, n_fre
     the stack free_pages in place, in the order of the sequences and their
     tables, and their table entries become -1.  Returns (context_lens, n_free):
     lengths with 0 for the finished ones, and the new number of free pages."""
+    out = _native().paged_release(block_table, context_lens, finished, free_pages, n_free, block_size)
+    if out is not None:
+        return out
     _check_tensors(block_table=block_table, context_lens=context_lens, finished=finished, free_pages=free_pages,
                    n_free=n_free)
     B, W = _check_maps(block_table, {"context_lens": context_lens, "finished": finished}, free_pages, n_free,
@@ -161,6 +167,10 @@ def sp2norm_paged_qk_norm_rope_append(q, k, v, q_weight, k_weight, cos, sin, pos
     caches, each rounded once to their type; a negative slot writes nothing.
     The slots of a call that are not negative must differ.  Returns the normed
     and rotated queries [N, Hq, D] (``[:, :, None]`` of them is a decode's q)."""
+    out = _native().paged_norm_append(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, eps,
+                                      block_size)
+    if out is not None:
+        return out
     _check_tensors(q=q, k=k, v=v, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin, positions=positions,
                    slots=slots, k_cache=k_cache, v_cache=v_cache)
     if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
@@ -231,6 +241,8 @@ def sp2norm_paged_key_bounds(k_cache, block_table, from_lens, to_lens, bounds=No
     smallest values, [:, :, 1] the largest, NaN where a key is.  All of a page's
     tokens below to_lens count, so a page that is filled step by step is right
     after each.  Table entries that name no page are skipped."""
+    if _native().paged_key_bounds(k_cache, block_table, from_lens, to_lens, bounds, block_size):
+        return bounds
     _check_tensors(k_cache=k_cache, block_table=block_table, from_lens=from_lens, to_lens=to_lens, bounds=bounds)
     if k_cache.ndim != 4:
         raise ValueError(f"k_cache must be [n_pages, H_kv, block_size, D], got {tuple(k_cache.shape)}")
@@ -272,6 +284,9 @@ def sp2norm_paged_select_pages(q, bounds, block_table, context_lens, top_k, *, n
     heads of q . k, computed in 64 bits (equal bounds: the lower page; NaN above
     all).  With n_last >= 1 the page that is being filled is always there, so
     its bounds may be behind."""
+    pages = _native().paged_select_pages(q, bounds, block_table, context_lens, top_k, n_first, n_last, block_size)
+    if pages is not None:
+        return pages
     _check_tensors(q=q, bounds=bounds, block_table=block_table, context_lens=context_lens)
     if q.ndim != 4 or q.shape[2] != 1:
         raise ValueError(f"q must be [B, H_q, 1, D], got {tuple(q.shape)}")
@@ -322,6 +337,9 @@ def sp2norm_paged_sparse_attention(q, k_cache, v_cache, block_table, context_len
     table are skipped, of a page the tokens below context_lens[b] count, and a
     page that is listed twice counts twice.  No token at all gives zeros.  The
     other arguments, types and head dims are sp2norm_paged_attention's."""
+    out = _native().paged_sparse(q, k_cache, v_cache, block_table, context_lens, pages, scale, block_size)
+    if out is not None:
+        return out
     _check_tensors(q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, context_lens=context_lens,
                    pages=pages)
     if q.ndim != 4 or q.shape[2] != 1:

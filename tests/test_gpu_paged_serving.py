@@ -141,6 +141,18 @@ def test_append_of_nothing_and_into_strided_caches():
     assert none.shape == (0, 4, D) and torch.equal(k2, kc)
 
 
+def test_append_without_pages_or_query_heads():
+    D = 32
+    cos, sin = torch.ones(8, 16, device=DEV), torch.zeros(8, 16, device=DEV)
+    k = _randn((3, 2, D), BF, 1).to(DEV)
+    i32 = torch.arange(3, dtype=torch.int32, device=DEV)
+    none = torch.zeros(0, 2, 16, D, dtype=BF, device=DEV)
+    out = smooth_attn.sp2norm_paged_qk_norm_rope_append(k, k, k, None, None, cos, sin, i32, i32, none, none)
+    kc, vc = torch.zeros(1, 2, 16, D, dtype=BF, device=DEV), torch.zeros(1, 2, 16, D, dtype=BF, device=DEV)
+    empty = smooth_attn.sp2norm_paged_qk_norm_rope_append(k[:, :0], k, k, None, None, cos, sin, i32, i32, kc, vc)
+    assert empty.shape == (3, 0, D) and torch.equal(kc[0, :, :3].transpose(0, 1), out) and torch.equal(vc[0, :, :3].transpose(0, 1), k)
+
+
 # ---------------------------------------------------------------------------
 # Bounds.
 # ---------------------------------------------------------------------------

@@ -202,6 +202,17 @@ def test_empty_inputs():
     assert torch.equal(w.grad, torch.zeros(32, device=DEV))
 
 
+def test_no_heads_on_one_side():
+    cos, sin = (t.to(DEV) for t in _tables(4, 32))
+    q, w = _randn((2, 3, 4, 32), torch.float32, 1).to(DEV).requires_grad_(True), torch.ones(32, device=DEV, requires_grad=True)
+    a, none = smooth_attn.sp2norm_qk_norm_rope(q, q[:, :0], w, w, cos, sin)
+    none2, b = smooth_attn.sp2norm_qk_norm_rope(q[:, :0], q, w, w, cos, sin)
+    assert none.shape == none2.shape == (2, 0, 4, 32) and torch.equal(a, b)
+    ga = torch.autograd.grad(a.square().sum() + none.sum(), (q, w))
+    gb = torch.autograd.grad(b.square().sum() + none2.sum(), (q, w))
+    assert all(torch.equal(x, y) for x, y in zip(ga, gb)) and ga[0].abs().sum() > 0
+
+
 def test_other_stream_and_repeatable():
     B, H, T, D = 2, 8, 500, 128
     q, k = (_randn((B, H, T, D), torch.bfloat16, s).to(DEV).requires_grad_(True) for s in (1, 2))
