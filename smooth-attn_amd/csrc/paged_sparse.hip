@@ -145,7 +145,7 @@ struct SelectParams {
     int64_t bt_stride;
     int B, Hq, Hkv, G, D, P, logP, max_pages, n_pages, K, n_first, n_last;
     int splits;  // waves that share the pages of a (sequence, KV head)
-    int lpp;     // lanes per page: a power of two
+    int qcode;
 };
 
 __device__ __forceinline__ int pages_of(const SelectParams& p, int b) {
@@ -153,11 +153,81 @@ __device__ __forceinline__ int pages_of(const SelectParams& p, int b) {
     return (ctx + p.P - 1) >> p.logP;
 }
 
-// Scores.  lpp lanes hold a page's 2 D bounds, NCH chunks each (the minima's
-// chunks first); the lane's parts of Q- or Q+ stay in registers, in 64 bits.
-template <typename QE, typename E, int NCH>
+// N query values from column d, in floats (N = 4, 8 or 16; rows of 16-byte multiples).
+template <int N>
+__device__ __forceinline__ void load_query(const void* row, int code, int d, float* f) {
+    if (code == SA_F32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const float*>(row) + d + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[i + j] = __uint_as_float(w[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + d + i);
+            const uint32_t ww[2] = {w.x, w.y};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[i + j] = code == SA_BF16 ? elem<bf16>(ww, j) : elem<f16>(ww, j);
+        }
+    }
+}
+
+// The value of the lane that differs from this one in bit BIT of its number
+// (4: and in the two below it).
+template <int BIT>
+__device__ __forceinline__ double from_other(double v) {
+    if constexpr (BIT >= 16) {
+        return __shfl_xor(v, BIT);
+    } else {
+        constexpr int ctrl = BIT == 1 ? 0xB1 : BIT == 2 ? 0x4E : BIT == 4 ? 0x141 : 0x128;
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const float lo = dpp_mov<ctrl>(__uint_as_float(static_cast<uint32_t>(u)));
+        const float hi = dpp_mov<ctrl>(__uint_as_float(static_cast<uint32_t>(u >> 32)));
+        return __builtin_bit_cast(double, static_cast<uint64_t>(__float_as_uint(hi)) << 32 | __float_as_uint(lo));
+    }
+}
+
+// Sums of COUNT values over groups of 2 BIT lanes.  While a lane has several
+// values, each of two partners keeps half of them and takes the other's part, so
+// COUNT sums cost about as many exchanges as two whole ones; what is left in v[0
+// .. max(1, COUNT / (2 BIT))) belongs to the value that first_value names.
+template <int BIT, int COUNT>
+__device__ __forceinline__ void group_sums(double* v) {
+    if constexpr (COUNT > 1) {
+        const bool upper = (threadIdx.x & BIT) != 0;
+#pragma unroll
+        for (int i = 0; i < COUNT / 2; ++i) {
+            const double keep = upper ? v[i + COUNT / 2] : v[i];
+            const double send = upper ? v[i] : v[i + COUNT / 2];
+            v[i] = keep + from_other<BIT>(send);
+        }
+    } else {
+        v[0] += from_other<BIT>(v[0]);
+    }
+    if constexpr (BIT > 1) group_sums<BIT / 2, COUNT / 2 < 1 ? 1 : COUNT / 2>(v);
+}
+template <int BIT, int COUNT>
+__device__ __forceinline__ int first_value() {
+    if constexpr (COUNT > 1 && BIT >= 1) {
+        const int mine = (threadIdx.x & BIT) != 0 ? COUNT / 2 : 0;
+        return mine + first_value<BIT / 2, COUNT / 2>();
+    } else {
+        return 0;
+    }
+}
+
+// Scores.  LPP lanes hold a page's 2 D bounds, NCH chunks each (the minima's
+// chunks first); the lane's parts of Q- and Q+ stay in registers, in 64 bits.  A
+// wave takes kBatch loads' pages at a time: their table entries are read a batch
+// ahead, their bounds all before the first is used, and their sums are added up
+// together.
+constexpr int kBatch = 8;
+template <typename E, int LPP, int NCH>
 __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
     constexpr int N = Chunk<E>::N;
+    constexpr int PER = 64 / LPP;  // pages of one load
     const int lane = threadIdx.x & 63;
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (unit >= static_cast<int64_t>(p.B) * p.Hkv * p.splits) return;
@@ -166,49 +236,73 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
     const int b = bh / p.Hkv, h = bh - b * p.Hkv;
     const int np = pages_of(p, b);
     if (np <= p.K) return;  // all of them are taken
+    int j0 = part * PER * kBatch;
+    if (j0 >= np) return;
+    const int step = p.splits * PER * kBatch;
     const int chunks = p.D / N;
-    const int sub = lane & (p.lpp - 1);
+    const int sub = lane & (LPP - 1), mine = lane / LPP;
+    const int32_t* trow = p.table + b * p.bt_stride;
+    int page[kBatch];
+    auto read_table = [&](int j) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) page[u] = trow[min(j + u * PER + mine, np - 1)];
+    };
+    read_table(j0);
     double qv[NCH][N];
     int off[NCH];
 #pragma unroll
     for (int u = 0; u < NCH; ++u) {
-        const int c = sub + u * p.lpp;
-        off[u] = c < 2 * chunks ? c * N : -1;
+        const int c = sub + u * LPP;
+        off[u] = min(c, 2 * chunks - 1) * N;
 #pragma unroll
         for (int i = 0; i < N; ++i) qv[u][i] = 0.0;
         if (c >= 2 * chunks) continue;
         const bool upper = c >= chunks;
         const int d0 = (upper ? c - chunks : c) * N;
         for (int g = 0; g < p.G; ++g) {
-            const QE* row = static_cast<const QE*>(p.q) + b * p.qs0 + (h * p.G + g) * p.qs1 + d0;
+            const int64_t row = b * p.qs0 + (h * p.G + g) * p.qs1;
+            float x[N];
+            load_query<N>(static_cast<const char*>(p.q) + row * (p.qcode == SA_F32 ? 4 : 2), p.qcode, d0, x);
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float x = to_f32(row[i]);
-                // (NaN stays in both)
-                qv[u][i] += upper ? (x < 0.f ? 0.f : x) : (x > 0.f ? 0.f : x);
-            }
+            for (int i = 0; i < N; ++i)  // (NaN stays in both)
+                qv[u][i] += upper ? (x[i] < 0.f ? 0.f : x[i]) : (x[i] > 0.f ? 0.f : x[i]);
         }
     }
-    const int per = 64 / p.lpp;  // pages at a time
-    const int32_t* trow = p.table + b * p.bt_stride;
+    const int64_t page_size = static_cast<int64_t>(p.Hkv) * 2 * p.D;
     const E* base = static_cast<const E*>(p.bounds) + static_cast<int64_t>(h) * 2 * p.D;
     double* out = p.scores + static_cast<int64_t>(bh) * p.max_pages;
-    for (int j0 = part * per; j0 < np; j0 += p.splits * per) {
-        const int j = j0 + lane / p.lpp;
-        const int page = j < np ? min(max(trow[j], 0), p.n_pages - 1) : -1;
-        double s = 0.0;
-        if (page >= 0) {
-            const E* src = base + static_cast<int64_t>(page) * p.Hkv * 2 * p.D;
+    constexpr int LEFT = kBatch / LPP < 1 ? 1 : kBatch / LPP;  // sums that a lane ends up with
+    const int u0 = first_value<LPP / 2, kBatch>();
+    for (; j0 < np; j0 += step) {
+        u32x4 w[kBatch][NCH];
 #pragma unroll
-            for (int u = 0; u < NCH; ++u) {
-                if (off[u] < 0) continue;
-                const Chunk<E> x = widen<E>(*reinterpret_cast<const u32x4*>(src + off[u]));
+        for (int u = 0; u < kBatch; ++u) {
+            const E* src = base + min(max(page[u], 0), p.n_pages - 1) * page_size;
 #pragma unroll
-                for (int i = 0; i < N; ++i) s = __builtin_fma(qv[u][i], static_cast<double>(x.f[i]), s);
+            for (int c = 0; c < NCH; ++c) w[u][c] = *reinterpret_cast<const u32x4*>(src + off[c]);
+        }
+        if (j0 + step < np) read_table(j0 + step);
+        double s[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            s[u] = 0.0;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                if (2 * chunks < LPP * NCH && sub + c * LPP >= 2 * chunks) continue;  // (no such chunk)
+                const Chunk<E> x = widen<E>(w[u][c]);
+#pragma unroll
+                for (int i = 0; i < N; ++i) s[u] = __builtin_fma(qv[c][i], static_cast<double>(x.f[i]), s[u]);
             }
         }
-        for (int o = 1; o < p.lpp; o <<= 1) s += __shfl_xor(s, o);
-        if (page >= 0 && sub == 0) out[j] = s;
+        group_sums<LPP / 2, kBatch>(s);
+        // (lanes below the last exchange hold the same sum: the lowest writes it)
+        if (LPP <= kBatch || (sub & (LPP / kBatch - 1)) == 0) {
+#pragma unroll
+            for (int i = 0; i < LEFT; ++i) {
+                const int j = j0 + (u0 + i) * PER + mine;
+                if (j < np) out[j] = s[i];
+            }
+        }
     }
 }
 
@@ -219,144 +313,246 @@ __device__ __forceinline__ uint64_t order_key(double s) {
     return (u >> 63) ? ~u : u | (1ull << 63);
 }
 
-constexpr int kPick = 512;   // threads of a choice
 constexpr int kBins = 2048;
-
-// Block sums of two counts in one word each (both below 2^31).
-struct Scan {
-    uint64_t before, total;
-};
-__device__ __forceinline__ Scan block_scan(uint64_t v, uint64_t* part) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    uint64_t x = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint64_t u = __shfl_up(x, off);
-        if (lane >= off) x += u;
-    }
-    __syncthreads();
-    if (lane == 63) part[wv] = x;
-    __syncthreads();
-    Scan s{x - v, 0};
-#pragma unroll
-    for (int i = 0; i < kPick / 64; ++i) {
-        if (i < wv) s.before += part[i];
-        s.total += part[i];
-    }
-    return s;
-}
+constexpr int kRanked = 256;  // keys that are ranked one against another
 
 // The pages of one (sequence, KV head): the first n_first, the last n_last and
-// the others with the largest scores, ascending.  The border score is found by
-// narrowing the range of keys that holds it, by a factor of up to kBins a pass:
-// a histogram of the range, and the bin in which the count from above reaches
-// what is needed.  Of equal scores at the border the lower pages are taken.
-__global__ __launch_bounds__(kPick) void paged_pick_kernel(SelectParams p) {
+// the others with the largest scores, ascending; of equal scores at the border
+// the lower pages.
+//
+// The border score is found by narrowing the range of keys that holds it: a
+// histogram of the range in LDS, and the bin in which the count from above
+// reaches what is needed, a factor of up to kBins a pass.  Once at most kRanked
+// keys are left they are ranked against each other (one pass and about ten keys
+// for a few thousand scores).  Pages are written in order: page j = KEYS-th i of
+// thread t is i * THREADS + t, so a wave's ballot is 64 pages in a row, and one
+// sum over the ballots' counts places them all.
+//
+// A thread keeps its keys in registers, all read at once: with every pass reading
+// them from memory, 512 lists of up to 1024 pages took 10.3 us and 64 of up to
+// 8192 30.5.  KEYS = 0: any number of pages, read in every pass.
+template <int THREADS, int KEYS>
+__global__ __launch_bounds__(THREADS) void paged_pick_kernel(SelectParams p) {
+    constexpr int WAVES = THREADS / 64;
     __shared__ uint32_t hist[kBins];
-    __shared__ uint64_t part[kPick / 64];
-    __shared__ uint64_t range[2];
-    __shared__ uint32_t found[2];
+    __shared__ uint64_t ranked[kRanked];
+    __shared__ uint32_t sums[2][WAVES];
+    __shared__ uint32_t found[4];  // bin, needed from it, keys in it; keys ranked so far
+    __shared__ uint64_t border_at;
+    __shared__ uint32_t ties_at;
     const int bh = blockIdx.x, tid = threadIdx.x;
+    const int lane = tid & 63, wv = tid >> 6;
     const int b = bh / p.Hkv;
     const int np = pages_of(p, b);
     int32_t* out = p.pages + static_cast<int64_t>(bh) * p.K;
     if (np <= p.K) {
-        for (int i = tid; i < p.K; i += kPick) out[i] = i < np ? i : -1;
+        for (int i = tid; i < p.K; i += THREADS) out[i] = i < np ? i : -1;
         return;
     }
     const double* scores = p.scores + static_cast<int64_t>(bh) * p.max_pages;
     const int first = p.n_first, last = np - p.n_last;  // (n_first + n_last <= K < np)
+    uint64_t mine[KEYS > 0 ? KEYS : 1];
+    if constexpr (KEYS > 0) {
+        double v[KEYS];
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) v[i] = scores[min(i * THREADS + tid, np - 1)];
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) mine[i] = order_key(v[i]);
+    }
+    // f(key) for the pages that compete
+    auto each = [&](auto f) {
+        if constexpr (KEYS > 0) {
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) {
+                const int j = i * THREADS + tid;
+                if (j >= first && j < last) f(mine[i]);
+            }
+        } else {
+            for (int j = first + tid; j < last; j += THREADS) f(order_key(scores[j]));
+        }
+    };
     uint32_t need = p.K - p.n_first - p.n_last;
     uint64_t border = ~0ull;
     uint32_t ties = 0;  // pages at the border to take
-    if (need > 0) {
-        // smallest and largest key
-        uint64_t lo = ~0ull, hi = 0;
-        for (int j = first + tid; j < last; j += kPick) {
-            const uint64_t k = order_key(scores[j]);
-            lo = smaller(lo, k);
-            hi = larger(hi, k);
-        }
+    bool some = need > 0;
+    if (some) {
+        uint64_t lo, hi;
+        {  // the range, from the keys' high halves
+            uint32_t least = ~0u, most = 0;
+            each([&](uint64_t k) {
+                least = smaller(least, static_cast<uint32_t>(k >> 32));
+                most = larger(most, static_cast<uint32_t>(k >> 32));
+            });
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            lo = smaller<uint64_t>(lo, __shfl_xor(lo, o));
-            hi = larger<uint64_t>(hi, __shfl_xor(hi, o));
+            for (int o = 1; o < 64; o <<= 1) {
+                least = smaller<uint32_t>(least, __shfl_xor(least, o));
+                most = larger<uint32_t>(most, __shfl_xor(most, o));
+            }
+            if (lane == 0) sums[0][wv] = least, sums[1][wv] = most;
+            for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+                least = smaller(least, sums[0][i]);
+                most = larger(most, sums[1][i]);
+            }
+            lo = static_cast<uint64_t>(least) << 32;
+            hi = static_cast<uint64_t>(most) << 32 | 0xFFFFFFFFu;
+            __syncthreads();
         }
-        if (tid == 0) range[0] = ~0ull, range[1] = 0;
-        __syncthreads();
-        if ((tid & 63) == 0) {
-            atomicMin(reinterpret_cast<unsigned long long*>(&range[0]), lo);
-            atomicMax(reinterpret_cast<unsigned long long*>(&range[1]), hi);
-        }
-        __syncthreads();
-        lo = range[0];
-        hi = range[1];
-        for (;;) {
-            const uint64_t width = hi - lo;
-            if (width == 0) {
+        for (;;) {  // hist is clear
+            const int shift = max(0, 64 - static_cast<int>(__builtin_clzll(hi - lo | 1)) - 11);
+            each([&](uint64_t k) {
+                if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
+            });
+            __syncthreads();
+            // thread t: the bins below those of thread t - 1, from the top
+            constexpr int PER = kBins / THREADS;
+            uint32_t count[PER], sum = 0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) sum += count[i] = hist[kBins - 1 - (tid * PER + i)];
+            uint32_t upto = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t u = __shfl_up(upto, o);
+                upto += lane >= o ? u : 0u;
+            }
+            if (lane == 63) sums[0][wv] = upto;
+            if (tid == 0) found[3] = 0;
+            __syncthreads();
+            uint32_t above = upto - sum;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) above += i < wv ? sums[0][i] : 0u;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                if (above < need && above + count[i] >= need) {  // (in one bin of one thread)
+                    found[0] = kBins - 1 - (tid * PER + i);
+                    found[1] = need - above;
+                    found[2] = count[i];
+                }
+                above += count[i];
+            }
+#pragma unroll
+            for (int i = 0; i < PER; ++i) hist[kBins - 1 - (tid * PER + i)] = 0;
+            __syncthreads();
+            need = found[1];
+            const uint32_t left = found[2];
+            lo += static_cast<uint64_t>(found[0]) << shift;
+            hi = lo + smaller<uint64_t>(hi - lo, (1ull << shift) - 1);  // (no sum past 64 bits)
+            if (left == need) {  // all keys from here up
+                border = lo - 1;
+                break;
+            }
+            if (lo == hi) {
                 border = lo;
                 ties = need;
                 break;
             }
-            const int shift = max(0, 64 - static_cast<int>(__builtin_clzll(width)) - 11);
-            for (int i = tid; i < kBins; i += kPick) hist[i] = 0;
-            __syncthreads();
-            for (int j = first + tid; j < last; j += kPick) {
-                const uint64_t k = order_key(scores[j]);
-                if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
-            }
-            __syncthreads();
-            // thread t: the kBins / kPick bins below those of thread t - 1, from the top
-            constexpr int kPer = kBins / kPick;
-            uint32_t mine = 0;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) mine += hist[kBins - 1 - (tid * kPer + i)];
-            const Scan s = block_scan(mine, part);
-            if (s.before < need && s.before + mine >= need) {
-                uint32_t above = static_cast<uint32_t>(s.before);
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    const uint32_t n = hist[kBins - 1 - (tid * kPer + i)];
-                    if (above < need && above + n >= need) {
-                        found[0] = kBins - 1 - (tid * kPer + i);
-                        found[1] = need - above;
-                        above = need;  // (no later bin)
-                    } else if (above < need) {
-                        above += n;
+            if (left <= kRanked) {
+                each([&](uint64_t k) {
+                    if (k >= lo && k <= hi) ranked[atomicAdd(&found[3], 1u)] = k;
+                });
+                __syncthreads();
+                for (uint32_t r = tid; r < left; r += THREADS) {
+                    const uint64_t k = ranked[r];
+                    uint32_t over = 0, same = 0;
+                    for (uint32_t i = 0; i < left; ++i) {
+                        over += ranked[i] > k;
+                        same += ranked[i] == k;
+                    }
+                    if (over < need && over + same >= need) {  // (equal keys say the same)
+                        border_at = k;
+                        ties_at = need - over;
                     }
                 }
-            }
-            __syncthreads();
-            const uint32_t bin = found[0];
-            need = found[1];
-            const uint64_t start = lo + (static_cast<uint64_t>(bin) << shift);
-            const bool whole = hist[bin] == need;
-            __syncthreads();
-            if (whole) {  // all keys from here up
-                border = start - 1;
+                __syncthreads();
+                border = border_at;
+                ties = ties_at;
                 break;
             }
-            hi = start + smaller<uint64_t>(hi - start, (1ull << shift) - 1);  // (no sum past 64 bits)
-            lo = start;
+            __syncthreads();  // found has been read
         }
     }
-    // In the order of the pages: those above the border, and of those at it the first ones.
-    uint64_t carry = 0;  // taken pages (low half), pages at the border (high half)
-    for (int j0 = 0; j0 < np; j0 += kPick) {
-        const int j = j0 + tid;
-        bool take = false, tie = false;
-        if (j < np) {
-            const bool always = j < first || j >= last;
-            const uint64_t k = always ? 0 : order_key(scores[j]);
-            take = always || (border != ~0ull && k > border);
-            tie = !always && ties > 0 && k == border;
+    // Which pages, and where: in the order of the pages, those above the border
+    // and the first of those at it.
+    auto choose = [&](int j, uint64_t k, bool& take, bool& tie) {
+        const bool always = j < first || (j >= last && j < np);
+        take = always || (some && j < last && k > border);
+        tie = !always && j < last && ties > 0 && k == border;
+    };
+    const uint64_t below = (1ull << lane) - 1;
+    if constexpr (KEYS > 0) {
+        __shared__ uint32_t words[2][KEYS * WAVES];
+        uint64_t takes[KEYS], tied[KEYS];
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) {
+            bool take, tie;
+            choose(i * THREADS + tid, mine[i], take, tie);
+            takes[i] = __ballot(take);
+            tied[i] = __ballot(tie);
+            if (lane == 0) {
+                words[0][i * WAVES + wv] = __popcll(takes[i]);
+                words[1][i * WAVES + wv] = __popcll(tied[i]);
+            }
         }
-        Scan s = block_scan((tie ? 1ull << 32 : 0) | (take ? 1 : 0), part);
-        s.before += carry;
-        const uint32_t tied_before = static_cast<uint32_t>(s.before >> 32);
-        const uint32_t at = static_cast<uint32_t>(s.before) + min(tied_before, ties);
-        if (take || (tie && tied_before < ties)) out[at] = j;
-        carry += s.total;
+        __syncthreads();
+        // every wave adds up the words for itself: lane l the run l of them
+        constexpr int RUN = (KEYS * WAVES + 63) / 64;
+        uint32_t sum[2] = {0, 0}, at[2][RUN];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) {
+                const int w = lane * RUN + i;
+                at[c][i] = sum[c];
+                sum[c] += w < KEYS * WAVES ? words[c][w] : 0u;
+            }
+            uint32_t upto = sum[c];
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t u = __shfl_up(upto, o);
+                upto += lane >= o ? u : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) at[c][i] += upto - sum[c];
+        }
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) {
+            const int w = i * WAVES + wv;
+            uint32_t before[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t v = 0;
+#pragma unroll
+                for (int r = 0; r < RUN; ++r) v = w % RUN == r ? __shfl(at[c][r], w / RUN) : v;
+                before[c] = v;
+            }
+            const bool take = takes[i] >> lane & 1, tie = tied[i] >> lane & 1;
+            const uint32_t t = before[1] + __popcll(tied[i] & below);
+            if (take || (tie && t < ties)) out[before[0] + __popcll(takes[i] & below) + smaller(t, ties)] = i * THREADS + tid;
+        }
+    } else {
+        uint32_t before[2] = {0, 0};
+        for (int j0 = 0; j0 < np; j0 += THREADS) {
+            const int j = j0 + tid;
+            bool take = false, tie = false;
+            if (j < np) choose(j, order_key(scores[j]), take, tie);
+            const uint64_t takes = __ballot(take), tied = __ballot(tie);
+            if (lane == 0) sums[0][wv] = __popcll(takes), sums[1][wv] = __popcll(tied);
+            __syncthreads();
+            uint32_t at[2] = {before[0], before[1]};
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    at[c] += i < wv ? sums[c][i] : 0u;
+                    before[c] += sums[c][i];
+                }
+            }
+            const uint32_t t = at[1] + __popcll(tied & below);
+            if (take || (tie && t < ties)) out[at[0] + __popcll(takes & below) + smaller(t, ties)] = j;
+            __syncthreads();
+        }
     }
 }
 
@@ -389,22 +585,24 @@ int splits_for(int64_t units, int64_t most) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, (256 * 16 + units - 1) / units)));
 }
 
-template <typename QE, typename E>
-int launch_scores(const SelectParams& p, int nch, unsigned blocks, hipStream_t st) {
-    switch (nch) {
-        case 1: paged_score_kernel<QE, E, 1><<<blocks, 256, 0, st>>>(p); break;
-        case 2: paged_score_kernel<QE, E, 2><<<blocks, 256, 0, st>>>(p); break;
-        case 4: paged_score_kernel<QE, E, 4><<<blocks, 256, 0, st>>>(p); break;
-        default: paged_score_kernel<QE, E, 8><<<blocks, 256, 0, st>>>(p); break;
+template <typename E>
+int launch_scores(const SelectParams& p, int lpp, int nch, unsigned blocks, hipStream_t st) {
+    switch (lpp * nch) {
+        case 2: paged_score_kernel<E, 2, 1><<<blocks, 256, 0, st>>>(p); break;
+        case 4: paged_score_kernel<E, 4, 1><<<blocks, 256, 0, st>>>(p); break;
+        case 8: paged_score_kernel<E, 8, 1><<<blocks, 256, 0, st>>>(p); break;
+        case 16: paged_score_kernel<E, 16, 1><<<blocks, 256, 0, st>>>(p); break;
+        case 32: paged_score_kernel<E, 32, 1><<<blocks, 256, 0, st>>>(p); break;
+        case 64: paged_score_kernel<E, 64, 1><<<blocks, 256, 0, st>>>(p); break;
+        case 128: paged_score_kernel<E, 64, 2><<<blocks, 256, 0, st>>>(p); break;
+        case 256:  // (head dims up to 1024: more chunks are of wider types)
+            if constexpr (sizeof(E) > 1) paged_score_kernel<E, 64, 4><<<blocks, 256, 0, st>>>(p);
+            break;
+        default:
+            if constexpr (sizeof(E) > 2) paged_score_kernel<E, 64, 8><<<blocks, 256, 0, st>>>(p);
+            break;
     }
     return status_from_launch();
-}
-template <typename QE>
-int launch_scores(const SelectParams& p, int cache, int nch, unsigned blocks, hipStream_t st) {
-    if (cache == SA_BF16) return launch_scores<QE, bf16>(p, nch, blocks, st);
-    if (cache == SA_F16) return launch_scores<QE, f16>(p, nch, blocks, st);
-    if (cache == SA_F32) return launch_scores<QE, float>(p, nch, blocks, st);
-    return launch_scores<QE, fp8e4>(p, nch, blocks, st);
 }
 
 // Listed tiles per wave at least: 16 (few partials) where the lists fill the
@@ -476,7 +674,8 @@ extern "C" int sa_paged_select_pages(const void* q, const void* bounds, const in
     if (B == 0 || top_k == 0) return 0;
     if (!q || !pages || !q_strides || !context_lens || (max_pages > 0 && (!bounds || !block_table)))
         return SA_ERR_NULL_POINTER;
-    if (q_strides[3] != 1 || !aligned16(bounds) || D % (16 / bytes_of(cache_dtype)) != 0) return SA_ERR_BAD_STRIDE;
+    const int q16 = dtype == SA_F32 ? 4 : 8;
+    if (q_strides[3] != 1 || q_strides[0] % q16 != 0 || q_strides[1] % q16 != 0 || !aligned16(q) || !aligned16(bounds) || D % (16 / bytes_of(cache_dtype)) != 0) return SA_ERR_BAD_STRIDE;
     const bool choose = top_k < max_pages && n_pages > 0;
     if (choose && (!workspace || workspace_bytes < sa_paged_select_workspace_size(B, Hkv, max_pages)))
         return SA_ERR_WORKSPACE;
@@ -502,20 +701,26 @@ extern "C" int sa_paged_select_pages(const void* q, const void* bounds, const in
     p.K = top_k;
     p.n_first = n_first;
     p.n_last = n_last;
+    p.qcode = dtype;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (choose) {
         const int chunks = 2 * D * bytes_of(cache_dtype) / 16;
-        p.lpp = std::min(64, pow2_up(chunks));
-        const int nch = pow2_up((chunks + p.lpp - 1) / p.lpp);
-        p.splits = splits_for(static_cast<int64_t>(B) * Hkv, (max_pages + 64 / p.lpp - 1) / (64 / p.lpp));
+        const int lpp = std::min(64, pow2_up(chunks)), nch = pow2_up((chunks + lpp - 1) / lpp);
+        const int batch = kBatch * (64 / lpp);  // pages that a wave takes at a time
+        p.splits = splits_for(static_cast<int64_t>(B) * Hkv, (max_pages + batch - 1) / batch);
         const int64_t units = static_cast<int64_t>(B) * Hkv * p.splits;
         const unsigned blocks = static_cast<unsigned>((units + 3) / 4);
-        const int status = dtype == SA_BF16  ? launch_scores<bf16>(p, cache_dtype, nch, blocks, st)
-                           : dtype == SA_F16 ? launch_scores<f16>(p, cache_dtype, nch, blocks, st)
-                                             : launch_scores<float>(p, cache_dtype, nch, blocks, st);
+        const int status = cache_dtype == SA_BF16  ? launch_scores<bf16>(p, lpp, nch, blocks, st)
+                           : cache_dtype == SA_F16 ? launch_scores<f16>(p, lpp, nch, blocks, st)
+                           : cache_dtype == SA_F32 ? launch_scores<float>(p, lpp, nch, blocks, st)
+                                                   : launch_scores<fp8e4>(p, lpp, nch, blocks, st);
         if (status != 0) return status;
     }
-    paged_pick_kernel<<<static_cast<unsigned>(B) * Hkv, kPick, 0, st>>>(p);
+    const unsigned lists = static_cast<unsigned>(B) * Hkv;
+    if (!choose || max_pages <= 512 * 2) paged_pick_kernel<512, 2><<<lists, 512, 0, st>>>(p);
+    else if (max_pages <= 512 * 8) paged_pick_kernel<512, 8><<<lists, 512, 0, st>>>(p);
+    else if (max_pages <= 1024 * 16) paged_pick_kernel<1024, 16><<<lists, 1024, 0, st>>>(p);
+    else paged_pick_kernel<1024, 0><<<lists, 1024, 0, st>>>(p);
     return status_from_launch();
 }
 

@@ -244,7 +244,7 @@ def test_select(Hq, Hkv, D, P, qt, ct, lens, top_k, n_first, n_last):
     assert torch.equal(got.cpu(), want)
 
 
-@pytest.mark.parametrize("np_", [3, 64, 513, 5000])
+@pytest.mark.parametrize("np_", [3, 64, 513, 1500, 5000, 17000])
 def test_select_ties_infinities_and_nan(np_):
     # a few distinct scores: the border falls inside a run of equal ones
     D, P = 8, 2
