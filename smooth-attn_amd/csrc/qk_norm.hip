@@ -60,33 +60,42 @@ struct NormParams {
     int T, D, n_pos, n_tokens, n_tiles, w32, page_size, n_pages;
 };
 
-// 8 consecutive elements.
-template <typename T>
+// 8 consecutive elements.  STREAM: past the caches (see streams()).
+template <bool STREAM>
+__device__ __forceinline__ u32x4 get16(const void* p) {
+    return STREAM ? load16(p) : *static_cast<const u32x4*>(p);
+}
+template <bool STREAM>
+__device__ __forceinline__ void put16(void* p, u32x4 v) {
+    if constexpr (STREAM) store16(p, v);
+    else *static_cast<u32x4*>(p) = v;
+}
+template <typename T, bool STREAM = false>
 __device__ __forceinline__ void load8(const T* p, float* f) {
+    const u32x4 a = get16<STREAM>(p);
     if constexpr (sizeof(T) == 4) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(p), b = *reinterpret_cast<const u32x4*>(p + 4);
+        const u32x4 b = get16<STREAM>(p + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             f[i] = __uint_as_float(a[i]);
             f[4 + i] = __uint_as_float(b[i]);
         }
     } else {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(p);
         const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = elem<T>(w, i);
     }
 }
-template <typename T>
+template <typename T, bool STREAM = false>
 __device__ __forceinline__ void store8(T* p, const float* f) {
     if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<u32x4*>(p) = u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                                             __float_as_uint(f[3])};
-        *reinterpret_cast<u32x4*>(p + 4) = u32x4{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
-                                                 __float_as_uint(f[7])};
+        put16<STREAM>(p, u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                               __float_as_uint(f[3])});
+        put16<STREAM>(p + 4, u32x4{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
+                                   __float_as_uint(f[7])});
     } else {
-        *reinterpret_cast<u32x4*>(p) = u32x4{pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]),
-                                             pack2<T>(f[6], f[7])};
+        put16<STREAM>(p, u32x4{pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]),
+                               pack2<T>(f[6], f[7])});
     }
 }
 
@@ -164,7 +173,7 @@ __device__ __forceinline__ int position_of(const NormParams& p, int b, int t) {
     return min(max(pos, 0), p.n_pos - 1);
 }
 
-template <typename T, int L, bool SERVE>
+template <typename T, int L, bool SERVE, bool STREAM>
 __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_kernel(NormParams p) {
     const int chunk = blockIdx.y;
     const int si = chunk >= p.first[2] ? 2 : chunk >= p.first[1] ? 1 : 0;
@@ -202,8 +211,8 @@ __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_kernel(NormParams 
     for (int h = h0 + at.h; h < h1; h += at.step) {
         float a[8], e[8];
         if (at.live) {
-            load8<T>(x + h * s.xs[1], a);
-            load8<T>(x + h * s.xs[1] + half, e);
+            load8<T, STREAM>(x + h * s.xs[1], a);
+            load8<T, STREAM>(x + h * s.xs[1] + half, e);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) a[i] = e[i] = 0.f;
@@ -232,8 +241,8 @@ __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_kernel(NormParams 
                 store8_cache(s.y, off, s.cache, ya);
                 store8_cache(s.y, off + half, s.cache, ye);
             } else {
-                store8<T>(static_cast<T*>(s.y) + off, ya);
-                store8<T>(static_cast<T*>(s.y) + off + half, ye);
+                store8<T, STREAM>(static_cast<T*>(s.y) + off, ya);
+                store8<T, STREAM>(static_cast<T*>(s.y) + off + half, ye);
             }
         }
     }
@@ -241,7 +250,7 @@ __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_kernel(NormParams 
 
 // Backward.  A wave keeps dw of its column pair over all its rows; a block adds
 // its waves' in a fixed order into its row of p.partial.
-template <typename T, int L>
+template <typename T, int L, bool STREAM>
 __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_bwd_kernel(NormParams p) {
     __shared__ float red[kBlockWaves][16 * L];
     const int chunk = blockIdx.y;
@@ -277,10 +286,10 @@ __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_bwd_kernel(NormPar
                 float a[8], e[8], ga[8], ge[8];
                 float sq = 0.f, hx = 0.f;
                 if (at.live) {
-                    load8<T>(x + h * s.xs[1], a);
-                    load8<T>(x + h * s.xs[1] + half, e);
-                    load8<T>(g + h * s.gs[1], ga);
-                    load8<T>(g + h * s.gs[1] + half, ge);
+                    load8<T, STREAM>(x + h * s.xs[1], a);
+                    load8<T, STREAM>(x + h * s.xs[1] + half, e);
+                    load8<T, STREAM>(g + h * s.gs[1], ga);
+                    load8<T, STREAM>(g + h * s.gs[1] + half, ge);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float zl = ga[i] * cv[i] + ge[i] * sv[i], zh = ge[i] * cv[i] - ga[i] * sv[i];
@@ -423,22 +432,24 @@ int by_type(int dtype, int lanes, A... a) {
 
 template <typename T, int L>
 struct LaunchFwd {
-    static int run(const NormParams& p, dim3 grid, hipStream_t st) {
-        norm_rope_kernel<T, L, false><<<grid, 64 * kBlockWaves, 0, st>>>(p);
+    static int run(const NormParams& p, dim3 grid, bool stream, hipStream_t st) {
+        if (stream) norm_rope_kernel<T, L, false, true><<<grid, 64 * kBlockWaves, 0, st>>>(p);
+        else norm_rope_kernel<T, L, false, false><<<grid, 64 * kBlockWaves, 0, st>>>(p);
         return status_from_launch();
     }
 };
 template <typename T, int L>
 struct LaunchServe {
     static int run(const NormParams& p, dim3 grid, hipStream_t st) {
-        norm_rope_kernel<T, L, true><<<grid, 64 * kBlockWaves, 0, st>>>(p);
+        norm_rope_kernel<T, L, true, false><<<grid, 64 * kBlockWaves, 0, st>>>(p);
         return status_from_launch();
     }
 };
 template <typename T, int L>
 struct LaunchBwd {
-    static int run(const NormParams& p, dim3 grid, hipStream_t st) {
-        norm_rope_bwd_kernel<T, L><<<grid, 64 * kBlockWaves, 0, st>>>(p);
+    static int run(const NormParams& p, dim3 grid, bool stream, hipStream_t st) {
+        if (stream) norm_rope_bwd_kernel<T, L, true><<<grid, 64 * kBlockWaves, 0, st>>>(p);
+        else norm_rope_bwd_kernel<T, L, false><<<grid, 64 * kBlockWaves, 0, st>>>(p);
         return status_from_launch();
     }
 };
@@ -491,10 +502,22 @@ void set_chunks(NormParams& p, const NormGrid& g, const int* heads, int sides) {
     for (int i = 0; i < 3; ++i) p.first[i + 1] = p.first[i] + (i < sides ? (heads[i] + g.CH - 1) / g.CH : 0);
 }
 
-// Blocks of the backward's grid along the tokens: as many partials as four
-// blocks on each CU make.
+// Blocks of the backward's grid along the tokens: about six on each CU in all
+// (the partials that they make are added up in 4 us), each with as many tiles as
+// the others.
 int64_t bwd_blocks(const NormGrid& g) {
-    return std::max<int64_t>(1, std::min<int64_t>(g.blocks, kCus * 4 / g.chunks));
+    const int64_t most = std::max<int64_t>(1, kCus * 6 / g.chunks);
+    const int64_t rounds = (g.blocks + most - 1) / most;
+    return (g.blocks + rounds - 1) / rounds;
+}
+
+// Whether a launch over this many rows of D elements goes past the caches: where
+// its tensors are larger than the last-level cache (256 MB), lines that nobody
+// reads again only push others out.  [4,32/32,4096,128] bf16 forward and
+// backward 274 -> 223 us; [2,32/8,1023,128] kernels 31.4 -> 33.9, so smaller
+// ones keep to the caches, where the next operator finds their results.
+bool streams(int64_t rows, int D, int dtype, int tensors) {
+    return rows * D * (dtype == SA_F32 ? 4 : 2) * tensors > (int64_t(256) << 20);
 }
 
 }  // namespace
@@ -533,7 +556,8 @@ extern "C" int sa_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, vo
     p.n_tokens = B * T;
     p.w32 = w_dtype == SA_F32;
     const dim3 grid(static_cast<unsigned>(g.blocks), static_cast<unsigned>(g.chunks));
-    return by_type<LaunchFwd>(dtype, g.lanes, p, grid, reinterpret_cast<hipStream_t>(stream));
+    const bool past = streams(static_cast<int64_t>(B) * T * (Hq + Hkv), D, dtype, 2);
+    return by_type<LaunchFwd>(dtype, g.lanes, p, grid, past, reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t sa_qk_norm_rope_bwd_workspace_size(int B, int Hq, int Hkv, int T, int D) {
@@ -592,7 +616,8 @@ extern "C" int sa_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_
     const int64_t blocks = bwd_blocks(g);
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(g.chunks));
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const int status = by_type<LaunchBwd>(dtype, g.lanes, p, grid, st);
+    const bool past = streams(static_cast<int64_t>(B) * T * (Hq + Hkv), D, dtype, 3);
+    const int status = by_type<LaunchBwd>(dtype, g.lanes, p, grid, past, st);
     if (status != 0 || !dw) return status;
     DwParams d{};
     d.partial[0] = workspace;

@@ -323,3 +323,25 @@ def test_training_step_replays_in_a_graph():
         want = step([t.clone().requires_grad_(True) for t in fresh])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+@pytest.mark.parametrize("dtype,B,T", [(torch.bfloat16, 2, 8192), (torch.float32, 2, 4096)])
+def test_tensors_past_the_caches(dtype, B, T):
+    # larger than the last-level cache: the same values as sequence by sequence, which is not
+    Hq, Hkv, D = 32, 8, 128
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, gq = (torch.randn(B, T, Hq, D, generator=g, device=DEV, dtype=dtype).transpose(1, 2) for _ in range(2))
+    k, gk = (torch.randn(B, T, Hkv, D, generator=g, device=DEV, dtype=dtype).transpose(1, 2) for _ in range(2))
+    w = 1 + 0.1 * torch.randn(D, generator=g, device=DEV)
+    cos, sin = (t.to(DEV) for t in _tables(T, D))
+
+    def step(rows):
+        args = [t[rows].detach().requires_grad_(True) for t in (q, k)] + [w.clone().requires_grad_(True) for _ in range(2)]
+        y = smooth_attn.sp2norm_qk_norm_rope(*args, cos, sin)
+        return [t.detach() for t in y] + list(torch.autograd.grad(y, args, (gq[rows], gk[rows])))
+
+    whole, parts = step(slice(0, B)), [step(slice(b, b + 1)) for b in range(B)]
+    for i in range(4):
+        assert all(torch.equal(whole[i][b:b + 1], parts[b][i]) for b in range(B)), i
+    for i in (4, 5):  # sums of 32-bit terms in another order
+        torch.testing.assert_close(whole[i], sum(p[i] for p in parts), rtol=1e-4, atol=1e-2)
