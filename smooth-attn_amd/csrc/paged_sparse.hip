@@ -58,9 +58,28 @@ __device__ __forceinline__ u32x4 narrow(const Chunk<E>& c) {
     return u32x4{w[0], w[1], w[2], w[3]};
 }
 
-// The smaller and the larger value; NaN where either is.
+// The smaller value; NaN where either is.
 __device__ __forceinline__ float min_nan(float a, float b) { return __builtin_elementwise_minimum(a, b); }
-__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Two registers with rows exchanged: of lanes that differ in BIT (16 or 32), the
+// lower ones get both values of a, the upper ones both of b (r.x from the lower
+// lane, r.y from the upper).
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int BIT>
+__device__ __forceinline__ u32x2 swap_rows(uint32_t a, uint32_t b) {
+    if constexpr (BIT == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+        return u32x2{r[0], r[1]};
+    } else {
+        const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+        return u32x2{r[0], r[1]};
+    }
+}
+template <int BIT>
+__device__ __forceinline__ float min_of_rows(float a, float b) {
+    const u32x2 r = swap_rows<BIT>(__float_as_uint(a), __float_as_uint(b));
+    return min_nan(__uint_as_float(r.x), __uint_as_float(r.y));
+}
 
 // ---------------------------------------------------------------------------
 // Bounds of the pages that hold tokens [from_b, to_b) of each sequence.
@@ -75,57 +94,82 @@ struct BoundsParams {
     int64_t bt_stride;
     int B, Hkv, D, P, logP, max_pages, n_pages;
     int splits;  // waves that share a (sequence, KV head)
-    int lpr;     // lanes per row: a power of two
 };
 
-// A wave takes every splits-th page of its (sequence, KV head): lpr lanes cover
-// a row (or 64 chunks of it at a time), 64 / lpr rows are read at once.
-template <typename E>
+// A wave takes every splits-th page of its (sequence, KV head): LPR lanes cover a
+// row (or 64 chunks of it at a time) and 64 / LPR rows are read at once, kAhead
+// such reads before the first is used.  Largest values are kept as smallest
+// negated ones, so both are the same operation: at the last exchange the lower
+// half of the wave takes over the one kind and the upper half the other.
+constexpr int kAhead = 4;
+template <typename E, int LPR>
 __global__ __launch_bounds__(256) void paged_bounds_kernel(BoundsParams p) {
     constexpr int N = Chunk<E>::N;
+    constexpr int ROWS = 64 / LPR;
     const int lane = threadIdx.x & 63;
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (unit >= static_cast<int64_t>(p.B) * p.Hkv * p.splits) return;
-    const int part = static_cast<int>(unit % p.splits);
-    const int bh = static_cast<int>(unit / p.splits);
+    const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (unit >= static_cast<uint32_t>(p.B * p.Hkv) * p.splits) return;
+    const int bh = unit / static_cast<uint32_t>(p.splits), part = unit - bh * p.splits;
     const int b = bh / p.Hkv, h = bh - b * p.Hkv;
     const int to = min(max(p.to[b], 0), p.max_pages << p.logP);
     const int from = max(p.from[b], 0);
     const int chunks = p.D / N;
-    const int row0 = lane / p.lpr, rows = 64 / p.lpr;
-    const float inf = __builtin_inff();
-    for (int j = (from >> p.logP) + part; (static_cast<int64_t>(j) << p.logP) < to; j += p.splits) {
-        const int page = p.table[b * p.bt_stride + j];
+    const int row0 = lane / LPR;
+    const int32_t* trow = p.table + b * p.bt_stride;
+    const int end = (to + p.P - 1) >> p.logP;
+    int j = (from >> p.logP) + part;
+    int next = j < end ? trow[j] : -1;
+    for (; j < end; j += p.splits) {
+        const int page = next;
+        if (j + p.splits < end) next = trow[j + p.splits];
         if (page < 0 || page >= p.n_pages) continue;
         const int n = min(to - (j << p.logP), p.P);
         const E* src = static_cast<const E*>(p.k) + page * p.ks[0] + h * p.ks[1];
         E* dst = static_cast<E*>(p.bounds) + (static_cast<int64_t>(page) * p.Hkv + h) * 2 * p.D;
-        for (int c0 = 0; c0 < chunks; c0 += p.lpr) {
-            const int c = c0 + (lane & (p.lpr - 1));
-            Chunk<E> lo, hi;
+        for (int c0 = 0; c0 < chunks; c0 += LPR) {
+            const int c = c0 + (lane & (LPR - 1));
+            const E* col = src + min(c, chunks - 1) * N;
+            float lo[N], hi[N];  // smallest values, and smallest negated ones
 #pragma unroll
-            for (int i = 0; i < N; ++i) lo.f[i] = inf, hi.f[i] = -inf;
-            if (c < chunks) {
-#pragma unroll 4
-                for (int r = row0; r < n; r += rows) {
-                    const Chunk<E> x = widen<E>(*reinterpret_cast<const u32x4*>(src + r * p.ks[2] + c * N));
+            for (int i = 0; i < N; ++i) lo[i] = hi[i] = __builtin_inff();
+            for (int r0 = 0; r0 < n; r0 += kAhead * ROWS) {
+                u32x4 w[kAhead];
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)  // (a row that is read twice changes nothing)
+                    w[a] = load16(col + min(r0 + a * ROWS + row0, n - 1) * p.ks[2]);
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) {
+                    const Chunk<E> x = widen<E>(w[a]);
 #pragma unroll
                     for (int i = 0; i < N; ++i) {
-                        lo.f[i] = min_nan(lo.f[i], x.f[i]);
-                        hi.f[i] = max_nan(hi.f[i], x.f[i]);
+                        lo[i] = min_nan(lo[i], x.f[i]);
+                        hi[i] = min_nan(hi[i], -x.f[i]);
                     }
                 }
             }
-            for (int o = p.lpr; o < 64; o <<= 1) {
+            Chunk<E> out;
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    lo.f[i] = min_nan(lo.f[i], __shfl_xor(lo.f[i], o));
-                    hi.f[i] = max_nan(hi.f[i], __shfl_xor(hi.f[i], o));
+            for (int i = 0; i < N; ++i) {
+                if constexpr (LPR <= 1) lo[i] = min_nan(lo[i], dpp_mov<0xB1>(lo[i])), hi[i] = min_nan(hi[i], dpp_mov<0xB1>(hi[i]));
+                if constexpr (LPR <= 2) lo[i] = min_nan(lo[i], dpp_mov<0x4E>(lo[i])), hi[i] = min_nan(hi[i], dpp_mov<0x4E>(hi[i]));
+                if constexpr (LPR <= 4) lo[i] = min_nan(lo[i], dpp_mov<0x124>(lo[i])), hi[i] = min_nan(hi[i], dpp_mov<0x124>(hi[i]));
+                if constexpr (LPR <= 8) lo[i] = min_nan(lo[i], dpp_mov<0x128>(lo[i])), hi[i] = min_nan(hi[i], dpp_mov<0x128>(hi[i]));
+                if constexpr (LPR <= 16) lo[i] = min_of_rows<16>(lo[i], lo[i]), hi[i] = min_of_rows<16>(hi[i], hi[i]);
+                if constexpr (LPR <= 32) {
+                    out.f[i] = min_of_rows<32>(lo[i], hi[i]);
+                    if (lane >= 32) out.f[i] = -out.f[i];
+                } else {
+                    out.f[i] = lo[i];
                 }
             }
-            if (row0 == 0 && c < chunks) {
-                *reinterpret_cast<u32x4*>(dst + c * N) = narrow<E>(lo);
-                *reinterpret_cast<u32x4*>(dst + p.D + c * N) = narrow<E>(hi);
+            if (c >= chunks) continue;
+            if constexpr (LPR <= 32) {
+                if ((lane & 31) < LPR) *reinterpret_cast<u32x4*>(dst + (lane >= 32 ? p.D : 0) + c * N) = narrow<E>(out);
+            } else {
+                *reinterpret_cast<u32x4*>(dst + c * N) = narrow<E>(out);
+#pragma unroll
+                for (int i = 0; i < N; ++i) out.f[i] = -hi[i];
+                *reinterpret_cast<u32x4*>(dst + p.D + c * N) = narrow<E>(out);
             }
         }
     }
@@ -195,7 +239,16 @@ __device__ __forceinline__ double from_other(double v) {
 // .. max(1, COUNT / (2 BIT))) belongs to the value that first_value names.
 template <int BIT, int COUNT>
 __device__ __forceinline__ void group_sums(double* v) {
-    if constexpr (COUNT > 1) {
+    if constexpr (COUNT > 1 && BIT >= 16) {
+#pragma unroll
+        for (int i = 0; i < COUNT / 2; ++i) {
+            const uint64_t a = __builtin_bit_cast(uint64_t, v[i]), b = __builtin_bit_cast(uint64_t, v[i + COUNT / 2]);
+            const u32x2 lo = swap_rows<BIT>(static_cast<uint32_t>(a), static_cast<uint32_t>(b));
+            const u32x2 hi = swap_rows<BIT>(static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b >> 32));
+            v[i] = __builtin_bit_cast(double, static_cast<uint64_t>(hi.x) << 32 | lo.x) +
+                   __builtin_bit_cast(double, static_cast<uint64_t>(hi.y) << 32 | lo.y);
+        }
+    } else if constexpr (COUNT > 1) {
         const bool upper = (threadIdx.x & BIT) != 0;
 #pragma unroll
         for (int i = 0; i < COUNT / 2; ++i) {
@@ -229,23 +282,22 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
     constexpr int N = Chunk<E>::N;
     constexpr int PER = 64 / LPP;  // pages of one load
     const int lane = threadIdx.x & 63;
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (unit >= static_cast<int64_t>(p.B) * p.Hkv * p.splits) return;
-    const int part = static_cast<int>(unit % p.splits);
-    const int bh = static_cast<int>(unit / p.splits);
+    const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (unit >= static_cast<uint32_t>(p.B * p.Hkv) * p.splits) return;
+    const int bh = unit / static_cast<uint32_t>(p.splits), part = unit - bh * p.splits;
     const int b = bh / p.Hkv, h = bh - b * p.Hkv;
-    const int np = pages_of(p, b);
-    if (np <= p.K) return;  // all of them are taken
     int j0 = part * PER * kBatch;
-    if (j0 >= np) return;
     const int step = p.splits * PER * kBatch;
     const int chunks = p.D / N;
     const int sub = lane & (LPP - 1), mine = lane / LPP;
+    // The length, the table entries and the queries are all read at once: entries
+    // past the sequence's pages are read, and not used.
     const int32_t* trow = p.table + b * p.bt_stride;
+    const int np = pages_of(p, b);
     int page[kBatch];
     auto read_table = [&](int j) {
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) page[u] = trow[min(j + u * PER + mine, np - 1)];
+        for (int u = 0; u < kBatch; ++u) page[u] = trow[min(j + u * PER + mine, p.max_pages - 1)];
     };
     read_table(j0);
     double qv[NCH][N];
@@ -259,15 +311,23 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
         if (c >= 2 * chunks) continue;
         const bool upper = c >= chunks;
         const int d0 = (upper ? c - chunks : c) * N;
-        for (int g = 0; g < p.G; ++g) {
-            const int64_t row = b * p.qs0 + (h * p.G + g) * p.qs1;
-            float x[N];
-            load_query<N>(static_cast<const char*>(p.q) + row * (p.qcode == SA_F32 ? 4 : 2), p.qcode, d0, x);
+        for (int g0 = 0; g0 < p.G; g0 += 4) {
+            float x[4][N];
 #pragma unroll
-            for (int i = 0; i < N; ++i)  // (NaN stays in both)
-                qv[u][i] += upper ? (x[i] < 0.f ? 0.f : x[i]) : (x[i] > 0.f ? 0.f : x[i]);
+            for (int g = 0; g < 4; ++g) {
+                const int64_t row = b * p.qs0 + (h * p.G + min(g0 + g, p.G - 1)) * p.qs1;
+                load_query<N>(static_cast<const char*>(p.q) + row * (p.qcode == SA_F32 ? 4 : 2), p.qcode, d0, x[g]);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (g0 + g >= p.G) continue;
+#pragma unroll
+                for (int i = 0; i < N; ++i)  // (NaN stays in both)
+                    qv[u][i] += upper ? (x[g][i] < 0.f ? 0.f : x[g][i]) : (x[g][i] > 0.f ? 0.f : x[g][i]);
+            }
         }
     }
+    if (np <= p.K) return;  // all of them are taken
     const int64_t page_size = static_cast<int64_t>(p.Hkv) * 2 * p.D;
     const E* base = static_cast<const E*>(p.bounds) + static_cast<int64_t>(h) * 2 * p.D;
     double* out = p.scores + static_cast<int64_t>(bh) * p.max_pages;
@@ -279,7 +339,7 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
         for (int u = 0; u < kBatch; ++u) {
             const E* src = base + min(max(page[u], 0), p.n_pages - 1) * page_size;
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) w[u][c] = *reinterpret_cast<const u32x4*>(src + off[c]);
+            for (int c = 0; c < NCH; ++c) w[u][c] = load16(src + off[c]);  // (past the caches: read once)
         }
         if (j0 + step < np) read_table(j0 + step);
         double s[kBatch];
@@ -306,11 +366,36 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
     }
 }
 
-// A score as an integer of the same order (NaN above all).
+// A score as an integer of the same order, above 2^32 (NaN above all).
 __device__ __forceinline__ uint64_t order_key(double s) {
-    if (!(s == s)) return ~0ull;
-    const uint64_t u = __builtin_bit_cast(uint64_t, s == 0.0 ? 0.0 : s);
-    return (u >> 63) ? ~u : u | (1ull << 63);
+    const uint64_t u = __builtin_bit_cast(uint64_t, s + 0.0);  // (-0 becomes 0)
+    const uint64_t m = static_cast<uint64_t>(static_cast<int64_t>(u) >> 63) | (1ull << 63);
+    return s == s ? u ^ m : ~0ull;
+}
+
+// Inclusive prefix sum, smallest and largest over the 64 lanes of a wave, by DPP:
+// rows of 16 first (row_shr, mirrors), then over the rows.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t old, uint32_t v) {
+    return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+    v += dpp_u32<0x111>(0, v);
+    v += dpp_u32<0x112>(0, v);
+    v += dpp_u32<0x114>(0, v);
+    v += dpp_u32<0x118>(0, v);
+    v += dpp_u32<0x142, 0xA>(0, v);  // row_bcast:15 into rows 1 and 3
+    v += dpp_u32<0x143, 0xC>(0, v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+template <typename F>
+__device__ __forceinline__ uint32_t wave_all(uint32_t v, F f) {
+    v = f(v, dpp_u32<0xB1>(v, v));
+    v = f(v, dpp_u32<0x4E>(v, v));
+    v = f(v, dpp_u32<0x141>(v, v));
+    v = f(v, dpp_u32<0x140>(v, v));
+    const auto at = [&](int l) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(v, l)); };
+    return f(f(at(0), at(16)), f(at(32), at(48)));
 }
 
 constexpr int kBins = 2048;
@@ -323,21 +408,26 @@ constexpr int kRanked = 256;  // keys that are ranked one against another
 // The border score is found by narrowing the range of keys that holds it: a
 // histogram of the range in LDS, and the bin in which the count from above
 // reaches what is needed, a factor of up to kBins a pass.  Once at most kRanked
-// keys are left they are ranked against each other (one pass and about ten keys
-// for a few thousand scores).  Pages are written in order: page j = KEYS-th i of
-// thread t is i * THREADS + t, so a wave's ballot is 64 pages in a row, and one
-// sum over the ballots' counts places them all.
+// keys are left they are ranked against each other (one pass, over the keys' high
+// halves, and about ten keys for a few thousand scores).  The pages taken are
+// bits in LDS, and the sums of their counts place them in order.
 //
-// A thread keeps its keys in registers, all read at once: with every pass reading
-// them from memory, 512 lists of up to 1024 pages took 10.3 us and 64 of up to
-// 8192 30.5.  KEYS = 0: any number of pages, read in every pass.
+// A thread keeps its keys in registers, all read at once.  One block's waves
+// share a CU, so what bounds this is the instructions for each key: with
+// compares of the position and of both ends of the range in 64 bits, and a
+// ballot for every 64 pages instead of the bits, 64 lists of up to 8192 pages
+// took 13.4 us, and with the keys read from memory in every pass 30.5.  KEYS = 0:
+// any number of pages, read in every pass.
 template <int THREADS, int KEYS>
 __global__ __launch_bounds__(THREADS) void paged_pick_kernel(SelectParams p) {
     constexpr int WAVES = THREADS / 64;
+    constexpr int WORDS = KEYS > 0 ? KEYS * THREADS / 32 : 1;
+    static_assert(WORDS <= THREADS, "a thread for each word of the bits");
     __shared__ uint32_t hist[kBins];
     __shared__ uint64_t ranked[kRanked];
     __shared__ uint32_t sums[2][WAVES];
-    __shared__ uint32_t found[4];  // bin, needed from it, keys in it; keys ranked so far
+    __shared__ uint32_t bits[2][WORDS];  // pages taken, pages at the border
+    __shared__ uint32_t found[4];        // bin, needed from it, keys in it; keys ranked so far
     __shared__ uint64_t border_at;
     __shared__ uint32_t ties_at;
     const int bh = blockIdx.x, tid = threadIdx.x;
@@ -345,95 +435,94 @@ __global__ __launch_bounds__(THREADS) void paged_pick_kernel(SelectParams p) {
     const int b = bh / p.Hkv;
     const int np = pages_of(p, b);
     int32_t* out = p.pages + static_cast<int64_t>(bh) * p.K;
+    const double* scores = p.scores + static_cast<int64_t>(bh) * p.max_pages;
+    double v[KEYS > 0 ? KEYS : 1];
+    if (KEYS > 0 && p.K < p.max_pages) {  // (else there are no scores; those past the sequence's pages are not used)
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) v[i] = scores[min(i * THREADS + tid, p.max_pages - 1)];
+    }
+    for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
+    if (tid < WORDS) bits[0][tid] = bits[1][tid] = 0;
     if (np <= p.K) {
         for (int i = tid; i < p.K; i += THREADS) out[i] = i < np ? i : -1;
         return;
     }
-    const double* scores = p.scores + static_cast<int64_t>(bh) * p.max_pages;
     const int first = p.n_first, last = np - p.n_last;  // (n_first + n_last <= K < np)
+    // Keys of the pages that compete, 0 for the others.
     uint64_t mine[KEYS > 0 ? KEYS : 1];
     if constexpr (KEYS > 0) {
-        double v[KEYS];
 #pragma unroll
-        for (int i = 0; i < KEYS; ++i) v[i] = scores[min(i * THREADS + tid, np - 1)];
-#pragma unroll
-        for (int i = 0; i < KEYS; ++i) mine[i] = order_key(v[i]);
+        for (int i = 0; i < KEYS; ++i) {
+            const int j = i * THREADS + tid;
+            mine[i] = j >= first && j < last ? order_key(v[i]) : 0;
+        }
     }
-    // f(key) for the pages that compete
     auto each = [&](auto f) {
         if constexpr (KEYS > 0) {
 #pragma unroll
             for (int i = 0; i < KEYS; ++i) {
-                const int j = i * THREADS + tid;
-                if (j >= first && j < last) f(mine[i]);
+                if (i * THREADS < np) f(mine[i], i * THREADS + tid);  // (the same for all threads)
             }
         } else {
-            for (int j = first + tid; j < last; j += THREADS) f(order_key(scores[j]));
+            for (int j = first + tid; j < last; j += THREADS) f(order_key(scores[j]), j);
         }
     };
     uint32_t need = p.K - p.n_first - p.n_last;
     uint64_t border = ~0ull;
     uint32_t ties = 0;  // pages at the border to take
-    bool some = need > 0;
-    if (some) {
-        uint64_t lo, hi;
-        {  // the range, from the keys' high halves
-            uint32_t least = ~0u, most = 0;
-            each([&](uint64_t k) {
-                least = smaller(least, static_cast<uint32_t>(k >> 32));
-                most = larger(most, static_cast<uint32_t>(k >> 32));
-            });
+    if (need > 0) {
+        // The range, from the keys' high halves (0 less 1 is the largest number).
+        uint32_t least = ~0u, most = 0;
+        each([&](uint64_t k, int) {
+            const uint32_t h = static_cast<uint32_t>(k >> 32);
+            least = smaller(least, h - 1);
+            most = larger(most, h);
+        });
+        least = wave_all(least, [](uint32_t x, uint32_t y) { return smaller(x, y); });
+        most = wave_all(most, [](uint32_t x, uint32_t y) { return larger(x, y); });
+        if (lane == 0) sums[0][wv] = least, sums[1][wv] = most;
+        __syncthreads();
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                least = smaller<uint32_t>(least, __shfl_xor(least, o));
-                most = larger<uint32_t>(most, __shfl_xor(most, o));
-            }
-            if (lane == 0) sums[0][wv] = least, sums[1][wv] = most;
-            for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < WAVES; ++i) {
-                least = smaller(least, sums[0][i]);
-                most = larger(most, sums[1][i]);
-            }
-            lo = static_cast<uint64_t>(least) << 32;
-            hi = static_cast<uint64_t>(most) << 32 | 0xFFFFFFFFu;
-            __syncthreads();
+        for (int i = 0; i < WAVES; ++i) {
+            least = smaller(least, sums[0][i]);
+            most = larger(most, sums[1][i]);
         }
-        for (;;) {  // hist is clear
-            const int shift = max(0, 64 - static_cast<int>(__builtin_clzll(hi - lo | 1)) - 11);
-            each([&](uint64_t k) {
-                if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
-            });
+        ++least;
+        uint64_t lo = static_cast<uint64_t>(least) << 32, hi = static_cast<uint64_t>(most) << 32 | 0xFFFFFFFFu;
+        int shift = 32 + max(0, 32 - static_cast<int>(__builtin_clz(most - least | 1)) - 11);
+        each([&](uint64_t k, int) {
+            const uint32_t h = static_cast<uint32_t>(k >> 32);
+            if (h != 0) atomicAdd(&hist[(h - least) >> (shift - 32)], 1u);
+        });
+        for (;;) {
             __syncthreads();
             // thread t: the bins below those of thread t - 1, from the top
             constexpr int PER = kBins / THREADS;
             uint32_t count[PER], sum = 0;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) sum += count[i] = hist[kBins - 1 - (tid * PER + i)];
-            uint32_t upto = sum;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t u = __shfl_up(upto, o);
-                upto += lane >= o ? u : 0u;
+            for (int i = 0; i < PER; ++i) {
+                uint32_t& bin = hist[kBins - 1 - (tid * PER + i)];
+                sum += count[i] = bin;
+                bin = 0;
             }
+            const uint32_t upto = wave_upto(sum);
             if (lane == 63) sums[0][wv] = upto;
             if (tid == 0) found[3] = 0;
             __syncthreads();
             uint32_t above = upto - sum;
 #pragma unroll
             for (int i = 0; i < WAVES; ++i) above += i < wv ? sums[0][i] : 0u;
+            if (above < need && above + sum >= need) {  // (one thread, one of its bins)
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                if (above < need && above + count[i] >= need) {  // (in one bin of one thread)
-                    found[0] = kBins - 1 - (tid * PER + i);
-                    found[1] = need - above;
-                    found[2] = count[i];
+                for (int i = 0; i < PER; ++i) {
+                    if (above < need && above + count[i] >= need) {
+                        found[0] = kBins - 1 - (tid * PER + i);
+                        found[1] = need - above;
+                        found[2] = count[i];
+                    }
+                    above += count[i];
                 }
-                above += count[i];
             }
-#pragma unroll
-            for (int i = 0; i < PER; ++i) hist[kBins - 1 - (tid * PER + i)] = 0;
             __syncthreads();
             need = found[1];
             const uint32_t left = found[2];
@@ -449,8 +538,8 @@ __global__ __launch_bounds__(THREADS) void paged_pick_kernel(SelectParams p) {
                 break;
             }
             if (left <= kRanked) {
-                each([&](uint64_t k) {
-                    if (k >= lo && k <= hi) ranked[atomicAdd(&found[3], 1u)] = k;
+                each([&](uint64_t k, int) {
+                    if (k - lo <= hi - lo) ranked[atomicAdd(&found[3], 1u)] = k;
                 });
                 __syncthreads();
                 for (uint32_t r = tid; r < left; r += THREADS) {
@@ -471,72 +560,57 @@ __global__ __launch_bounds__(THREADS) void paged_pick_kernel(SelectParams p) {
                 break;
             }
             __syncthreads();  // found has been read
+            shift = max(0, 64 - static_cast<int>(__builtin_clzll(hi - lo)) - 11);
+            each([&](uint64_t k, int) {
+                if (k - lo <= hi - lo) atomicAdd(&hist[(k - lo) >> shift], 1u);
+            });
         }
     }
-    // Which pages, and where: in the order of the pages, those above the border
-    // and the first of those at it.
-    auto choose = [&](int j, uint64_t k, bool& take, bool& tie) {
-        const bool always = j < first || (j >= last && j < np);
-        take = always || (some && j < last && k > border);
-        tie = !always && j < last && ties > 0 && k == border;
-    };
-    const uint64_t below = (1ull << lane) - 1;
+    // Which pages, and where: those above the border, the first of those at it,
+    // and the first and last ones.
     if constexpr (KEYS > 0) {
-        __shared__ uint32_t words[2][KEYS * WAVES];
-        uint64_t takes[KEYS], tied[KEYS];
-#pragma unroll
-        for (int i = 0; i < KEYS; ++i) {
-            bool take, tie;
-            choose(i * THREADS + tid, mine[i], take, tie);
-            takes[i] = __ballot(take);
-            tied[i] = __ballot(tie);
-            if (lane == 0) {
-                words[0][i * WAVES + wv] = __popcll(takes[i]);
-                words[1][i * WAVES + wv] = __popcll(tied[i]);
-            }
+        if (need == 0) __syncthreads();  // (the bits are clear)
+        each([&](uint64_t k, int j) {
+            if (k > border) atomicOr(&bits[0][j >> 5], 1u << (j & 31));
+        });
+        if (ties > 0)
+            each([&](uint64_t k, int j) {
+                if (k == border) atomicOr(&bits[1][j >> 5], 1u << (j & 31));
+            });
+        for (int i = tid; i < p.n_first + p.n_last; i += THREADS) {
+            const int j = i < first ? i : last + i - first;
+            atomicOr(&bits[0][j >> 5], 1u << (j & 31));
         }
         __syncthreads();
-        // every wave adds up the words for itself: lane l the run l of them
-        constexpr int RUN = (KEYS * WAVES + 63) / 64;
-        uint32_t sum[2] = {0, 0}, at[2][RUN];
+        // Sum over the words before this thread's.
+        auto before = [&](uint32_t n, uint32_t* part) {
+            const uint32_t upto = wave_upto(n);
+            if (lane == 63) part[wv] = upto;
+            __syncthreads();
+            uint32_t all = upto - n;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) {
-                const int w = lane * RUN + i;
-                at[c][i] = sum[c];
-                sum[c] += w < KEYS * WAVES ? words[c][w] : 0u;
+            for (int i = 0; i < (WORDS + 63) / 64; ++i) all += i < wv ? part[i] : 0u;
+            return all;
+        };
+        uint32_t word = tid < WORDS ? bits[0][tid] : 0u;
+        if (ties > 0) {
+            uint32_t tied = tid < WORDS ? bits[1][tid] : 0u;
+            const uint32_t done = before(__popc(tied), sums[0]);
+            for (uint32_t n = done; n < ties && tied != 0; ++n) {
+                word |= tied & (0u - tied);
+                tied &= tied - 1;
             }
-            uint32_t upto = sum[c];
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t u = __shfl_up(upto, o);
-                upto += lane >= o ? u : 0u;
-            }
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) at[c][i] += upto - sum[c];
         }
-#pragma unroll
-        for (int i = 0; i < KEYS; ++i) {
-            const int w = i * WAVES + wv;
-            uint32_t before[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t v = 0;
-#pragma unroll
-                for (int r = 0; r < RUN; ++r) v = w % RUN == r ? __shfl(at[c][r], w / RUN) : v;
-                before[c] = v;
-            }
-            const bool take = takes[i] >> lane & 1, tie = tied[i] >> lane & 1;
-            const uint32_t t = before[1] + __popcll(tied[i] & below);
-            if (take || (tie && t < ties)) out[before[0] + __popcll(takes[i] & below) + smaller(t, ties)] = i * THREADS + tid;
-        }
+        uint32_t at = before(__popc(word), sums[1]);
+        for (; word != 0; word &= word - 1) out[at++] = tid * 32 + __builtin_ctz(word);
     } else {
         uint32_t before[2] = {0, 0};
+        const uint64_t below = (1ull << lane) - 1;
         for (int j0 = 0; j0 < np; j0 += THREADS) {
             const int j = j0 + tid;
-            bool take = false, tie = false;
-            if (j < np) choose(j, order_key(scores[j]), take, tie);
+            const bool always = j < first || (j >= last && j < np);
+            const uint64_t k = !always && j < last ? order_key(scores[j]) : 0;
+            const bool take = always || k > border, tie = ties > 0 && k == border;
             const uint64_t takes = __ballot(take), tied = __ballot(tie);
             if (lane == 0) sums[0][wv] = __popcll(takes), sums[1][wv] = __popcll(tied);
             __syncthreads();
@@ -583,6 +657,20 @@ int check_pages(int B, int Hkv, int D, int page_size, int max_pages, int n_pages
 // Waves for each of `units`: as many as fill 16 waves a CU, at most `most`.
 int splits_for(int64_t units, int64_t most) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, (256 * 16 + units - 1) / units)));
+}
+
+template <typename E>
+int launch_bounds(const BoundsParams& p, int lpr, unsigned blocks, hipStream_t st) {
+    switch (lpr) {
+        case 1: paged_bounds_kernel<E, 1><<<blocks, 256, 0, st>>>(p); break;
+        case 2: paged_bounds_kernel<E, 2><<<blocks, 256, 0, st>>>(p); break;
+        case 4: paged_bounds_kernel<E, 4><<<blocks, 256, 0, st>>>(p); break;
+        case 8: paged_bounds_kernel<E, 8><<<blocks, 256, 0, st>>>(p); break;
+        case 16: paged_bounds_kernel<E, 16><<<blocks, 256, 0, st>>>(p); break;
+        case 32: paged_bounds_kernel<E, 32><<<blocks, 256, 0, st>>>(p); break;
+        default: paged_bounds_kernel<E, 64><<<blocks, 256, 0, st>>>(p); break;
+    }
+    return status_from_launch();
 }
 
 template <typename E>
@@ -642,16 +730,15 @@ extern "C" int sa_paged_key_bounds(const void* k_cache, void* bounds, const int3
     p.logP = log2_of(page_size);
     p.max_pages = max_pages;
     p.n_pages = n_pages;
-    p.lpr = std::min(64, pow2_up(D / n));
     p.splits = splits_for(static_cast<int64_t>(B) * Hkv, max_pages);
     const int64_t units = static_cast<int64_t>(B) * Hkv * p.splits;
     const unsigned blocks = static_cast<unsigned>((units + 3) / 4);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (cache_dtype == SA_BF16) paged_bounds_kernel<bf16><<<blocks, 256, 0, st>>>(p);
-    else if (cache_dtype == SA_F16) paged_bounds_kernel<f16><<<blocks, 256, 0, st>>>(p);
-    else if (cache_dtype == SA_F32) paged_bounds_kernel<float><<<blocks, 256, 0, st>>>(p);
-    else paged_bounds_kernel<fp8e4><<<blocks, 256, 0, st>>>(p);
-    return status_from_launch();
+    const int lpr = std::min(64, pow2_up(D / n));
+    if (cache_dtype == SA_BF16) return launch_bounds<bf16>(p, lpr, blocks, st);
+    if (cache_dtype == SA_F16) return launch_bounds<f16>(p, lpr, blocks, st);
+    if (cache_dtype == SA_F32) return launch_bounds<float>(p, lpr, blocks, st);
+    return launch_bounds<fp8e4>(p, lpr, blocks, st);
 }
 
 extern "C" int64_t sa_paged_select_workspace_size(int B, int Hkv, int max_pages) {
