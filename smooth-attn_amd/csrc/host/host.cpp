@@ -31,6 +31,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/version.h>
 
+#include <array>
 #include <cmath>
 #include <cstring>
 #include <memory>
@@ -778,6 +779,25 @@ PyObject* py_paged_norm_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// int32 vectors of the given sizes in one allocation, each from a multiple of
+// 256 bytes on: an allocation costs about as much host time as half a launch.
+template <size_t N>
+std::array<Tensor, N> int_vectors(const int64_t (&sizes)[N], const Tensor& like) {
+    constexpr int64_t step = 64;
+    int64_t total = 0;
+    for (int64_t n : sizes) total += (n + step - 1) / step * step;
+    const Tensor all = at::empty({total}, like.options().requires_grad(false));
+    std::array<Tensor, N> out;
+    int64_t at_element = 0;
+    for (size_t i = 0; i < N; ++i) {
+        out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+        out[i].unsafeGetTensorImpl()->set_storage_offset(at_element);
+        out[i].unsafeGetTensorImpl()->set_sizes_contiguous({sizes[i]});
+        at_element += (sizes[i] + step - 1) / step * step;
+    }
+    return out;
+}
+
 // What reserve and release take as they are: a table of B rows, lengths [B],
 // the stack and its count.
 bool maps_ok(const Tensor& table, const Tensor& lens, const Tensor& free_pages, const Tensor& n_free, int block_size) {
@@ -799,12 +819,11 @@ PyObject* py_paged_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !maps_ok(*table, *lens, *free_pages, *n_free, block_size) || !ints_ok(*fresh, table->size(0), *table) ||
         fresh->size(0) != table->size(0))
         Py_RETURN_NONE;
-    Tensor out[6];
+    std::array<Tensor, 6> out;
     {
         const NoGil released;
         const int64_t B = table->size(0);
-        const int64_t sizes[6] = {n_tokens, n_tokens, n_tokens, B + 1, B, 1};
-        for (int i = 0; i < 6; ++i) out[i] = at::empty({sizes[i]}, table->options());
+        out = int_vectors({n_tokens, n_tokens, n_tokens, B + 1, B, 1}, *table);
         const c10::DeviceGuard guard(table->device());
         const auto p = [](const Tensor& t) { return t.data_ptr<int32_t>(); };
         check(abi.paged_reserve(p(*table), p(*lens), p(*fresh), p(*free_pages), p(*n_free), p(out[0]), p(out[1]),
@@ -834,9 +853,10 @@ PyObject* py_paged_release(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
         const NoGil released;
         const int64_t B = table->size(0);
-        out = at::empty({B}, table->options());
-        left = at::empty({1}, table->options());
-        counts = at::empty({B}, table->options());
+        const auto made = int_vectors({B, 1, B}, *table);
+        out = made[0];
+        left = made[1];
+        counts = made[2];
         const c10::DeviceGuard guard(table->device());
         const auto p = [](const Tensor& t) { return t.data_ptr<int32_t>(); };
         check(abi.paged_release(p(*table), p(*lens), static_cast<const uint8_t*>(finished->data_ptr()), p(*free_pages),

@@ -157,21 +157,48 @@ __device__ __forceinline__ int pages_of(const ReleaseParams& p, int b) {
     return static_cast<int>((smaller<int64_t>(larger<int64_t>(p.ctx[b], 0), cap) + p.P - 1) / p.P);
 }
 
-__global__ __launch_bounds__(64) void paged_release_count_kernel(ReleaseParams p) {
-    const int b = blockIdx.x, lane = threadIdx.x;
-    const int n = pages_of(p, b);
-    int found = 0;
-    for (int j0 = 0; j0 < n; j0 += 64) {
-        const int j = j0 + lane;
-        const int page = j < n ? p.table[b * p.bt_stride + j] : -1;
-        found += __popcll(__ballot(page >= 0 && page < p.n_pages));
+// A block takes a sequence, kRun entries a thread at once: waiting for a table
+// of 1024 entries 64 at a time made 7 us of either kernel.
+constexpr int kRun = 4;
+
+__device__ __forceinline__ void read_entries(const ReleaseParams& p, int b, int j0, int n, int* page) {
+    const int32_t* row = p.table + b * p.bt_stride;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const int j = j0 + i * kThreads + static_cast<int>(threadIdx.x);
+        page[i] = j < n ? row[j] : -1;
     }
-    if (lane == 0) p.counts[b] = found;
 }
 
-__global__ __launch_bounds__(64) void paged_release_kernel(ReleaseParams p) {
-    const int b = blockIdx.x, lane = threadIdx.x;
+__global__ __launch_bounds__(kThreads) void paged_release_count_kernel(ReleaseParams p) {
+    __shared__ int part[kThreads / 64];
+    const int b = blockIdx.x;
     const int n = pages_of(p, b);
+    int found = 0;  // of the wave
+    for (int j0 = 0; j0 < n; j0 += kRun * kThreads) {
+        int page[kRun];
+        read_entries(p, b, j0, n, page);
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) found += __popcll(__ballot(page[i] >= 0 && page[i] < p.n_pages));
+    }
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = found;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int all = 0;
+#pragma unroll
+        for (int i = 0; i < kThreads / 64; ++i) all += part[i];
+        p.counts[b] = all;
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void paged_release_kernel(ReleaseParams p) {
+    __shared__ int words[kRun * kThreads / 64];  // pages given back in each 64 entries
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int n = pages_of(p, b);
+    if (n == 0 && b != 0) {  // (the first block also says how many pages there are)
+        if (threadIdx.x == 0) p.lens[b] = p.finished[b] ? 0 : p.ctx[b];
+        return;
+    }
     int64_t before = 0, all = 0;  // pages of the sequences before this one, and of all
     for (int i = lane; i < p.B; i += 64) {
         const int c = p.counts[i];
@@ -184,20 +211,36 @@ __global__ __launch_bounds__(64) void paged_release_kernel(ReleaseParams p) {
         all += __shfl_xor(all, o);
     }
     const int base = min(max(p.n_free[0], 0), p.n_pages);
-    if (lane == 0) {
+    if (threadIdx.x == 0) {
         p.lens[b] = p.finished[b] ? 0 : p.ctx[b];
         if (b == 0) p.n_free_out[0] = static_cast<int32_t>(smaller<int64_t>(base + all, p.n_pages));
     }
     int64_t at = base + before;
-    for (int j0 = 0; j0 < n; j0 += 64) {
-        const int j = j0 + lane;
-        const int page = j < n ? p.table[b * p.bt_stride + j] : -1;
-        const bool back = page >= 0 && page < p.n_pages;
-        const unsigned long long m = __ballot(back);
-        const int64_t to = at + __popcll(m & ((1ull << lane) - 1));
-        if (back && to < p.n_pages) p.free_pages[to] = page;
-        if (j < n) p.table[b * p.bt_stride + j] = -1;
-        at += __popcll(m);
+    for (int j0 = 0; j0 < n; j0 += kRun * kThreads) {
+        int page[kRun];
+        read_entries(p, b, j0, n, page);
+        unsigned long long back[kRun];
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+            back[i] = __ballot(page[i] >= 0 && page[i] < p.n_pages);
+            if (lane == 0) words[i * (kThreads / 64) + wv] = __popcll(back[i]);
+        }
+        __syncthreads();
+        int64_t to[kRun], sum = 0;
+#pragma unroll
+        for (int w = 0; w < kRun * kThreads / 64; ++w) {  // (the words are in the entries' order)
+            if (w % (kThreads / 64) == wv) to[w / (kThreads / 64)] = at + sum;
+            sum += words[w];
+        }
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+            const int j = j0 + i * kThreads + static_cast<int>(threadIdx.x);
+            const int64_t slot = to[i] + __popcll(back[i] & ((1ull << lane) - 1));
+            if ((back[i] >> lane & 1) && slot < p.n_pages) p.free_pages[slot] = page[i];
+            if (j < n) p.table[b * p.bt_stride + j] = -1;
+        }
+        at += sum;
+        __syncthreads();  // (words have been read)
     }
 }
 
@@ -274,9 +317,9 @@ extern "C" int sa_paged_release(int32_t* block_table, const int32_t* context_len
     p.P = page_size;
     p.n_pages = n_pages;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    paged_release_count_kernel<<<static_cast<unsigned>(B), 64, 0, st>>>(p);
+    paged_release_count_kernel<<<static_cast<unsigned>(B), kThreads, 0, st>>>(p);
     const int status = status_from_launch();
     if (status != 0) return status;
-    paged_release_kernel<<<static_cast<unsigned>(B), 64, 0, st>>>(p);
+    paged_release_kernel<<<static_cast<unsigned>(B), kThreads, 0, st>>>(p);
     return status_from_launch();
 }
