@@ -357,6 +357,11 @@ __global__ __launch_bounds__(64 * WPB) void paged_partial_kernel(PagedParams p) 
                     page_id = lane < npg ? min(max(trow[first_page + lane], 0), p.n_pages - 1) : 0;
                 }
             }
+            int t_stop = we;
+            if constexpr (Plan::LISTED) {  // (a list ends in pages that are none)
+                const unsigned long long some = __ballot(page_rows > 0);
+                t_stop = some == 0 ? ws : min(we, (first_page + 64 - __builtin_clzll(some)) << logP);
+            }
             // Bit r: token t0 + r of the tile at t0 is attended to (listed pages).
             auto tile_tokens = [&](int t0) {
                 const int t = t0 + l32;
@@ -444,14 +449,14 @@ __global__ __launch_bounds__(64 * WPB) void paged_partial_kernel(PagedParams p) 
             };
 
             load_tile(ws);
-            for (int t0 = ws; t0 < we; t0 += kTile) {
+            for (int t0 = ws; t0 < t_stop; t0 += kTile) {
                 // The block is one wavefront: LDS accesses of a wave complete
                 // in issue order, so a wave-level scheduling barrier is all
                 // the ordering needed.
                 store_tile();
                 __builtin_amdgcn_wave_barrier();
                 tokens = next_tokens;
-                if (t0 + kTile < we) load_tile(t0 + kTile);
+                if (t0 + kTile < t_stop) load_tile(t0 + kTile);
 
                 f32x16 s = f32x16{};
 #pragma unroll

@@ -58,9 +58,6 @@ __device__ __forceinline__ u32x4 narrow(const Chunk<E>& c) {
     return u32x4{w[0], w[1], w[2], w[3]};
 }
 
-// The smaller value; NaN where either is.
-__device__ __forceinline__ float min_nan(float a, float b) { return __builtin_elementwise_minimum(a, b); }
-
 // Two registers with rows exchanged: of lanes that differ in BIT (16 or 32), the
 // lower ones get both values of a, the upper ones both of b (r.x from the lower
 // lane, r.y from the upper).
@@ -75,11 +72,69 @@ __device__ __forceinline__ u32x2 swap_rows(uint32_t a, uint32_t b) {
         return u32x2{r[0], r[1]};
     }
 }
-template <int BIT>
-__device__ __forceinline__ float min_of_rows(float a, float b) {
-    const u32x2 r = swap_rows<BIT>(__float_as_uint(a), __float_as_uint(b));
-    return min_nan(__uint_as_float(r.x), __uint_as_float(r.y));
-}
+
+// The values of a 16-byte chunk as the bounds compare them: fp32 for fp32 and
+// bf16 keys, pairs of fp16 for fp16 and e4m3fn ones (each such value is an fp16
+// value), which gfx950 compares two at a time.
+template <typename E>
+struct Compared {
+    static constexpr bool PAIRS = std::is_same_v<E, f16> || std::is_same_v<E, fp8e4>;
+    using V = std::conditional_t<PAIRS, f16x2, float>;
+    static constexpr int N = PAIRS ? Chunk<E>::N / 2 : Chunk<E>::N;
+    // (by value: a cast of an element of a vector takes the first one)
+    static __device__ __forceinline__ f16x2 pair(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
+    static __device__ __forceinline__ void read(u32x4 w, V* v) {
+        if constexpr (std::is_same_v<E, f16>) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = pair(w[i]);
+        } else if constexpr (PAIRS) {
+            u32x4 lo, hi;
+            widen_e4m3x16<f16>(w, lo, hi);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = pair(lo[i]);
+                v[4 + i] = pair(hi[i]);
+            }
+        } else {
+            const Chunk<E> c = widen<E>(w);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = c.f[i];
+        }
+    }
+    static __device__ __forceinline__ u32x4 write(const V* v) {  // (exact)
+        if constexpr (std::is_same_v<E, f16>) {
+            return u32x4{__builtin_bit_cast(uint32_t, v[0]), __builtin_bit_cast(uint32_t, v[1]),
+                         __builtin_bit_cast(uint32_t, v[2]), __builtin_bit_cast(uint32_t, v[3])};
+        } else {
+            Chunk<E> c;
+            if constexpr (PAIRS) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    c.f[2 * i] = static_cast<float>(v[i][0]);
+                    c.f[2 * i + 1] = static_cast<float>(v[i][1]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) c.f[i] = v[i];
+            }
+            return narrow<E>(c);
+        }
+    }
+    static __device__ __forceinline__ V largest() {
+        if constexpr (PAIRS) return __builtin_bit_cast(f16x2, 0x7C007C00u);  // infinity
+        else return __builtin_inff();
+    }
+    static __device__ __forceinline__ V smaller_of(V a, V b) { return __builtin_elementwise_minimum(a, b); }  // (NaN stays)
+    template <int CTRL>
+    static __device__ __forceinline__ V moved(V v) {
+        return __builtin_bit_cast(V, dpp_mov<CTRL>(__builtin_bit_cast(float, v)));
+    }
+    template <int BIT>
+    static __device__ __forceinline__ V over_rows(V a, V b) {
+        const u32x2 r = swap_rows<BIT>(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+        return smaller_of(__builtin_bit_cast(V, static_cast<uint32_t>(r.x)), __builtin_bit_cast(V, static_cast<uint32_t>(r.y)));
+    }
+};
 
 // ---------------------------------------------------------------------------
 // Bounds of the pages that hold tokens [from_b, to_b) of each sequence.
@@ -104,6 +159,8 @@ struct BoundsParams {
 constexpr int kAhead = 4;
 template <typename E, int LPR>
 __global__ __launch_bounds__(256) void paged_bounds_kernel(BoundsParams p) {
+    using C = Compared<E>;
+    using V = typename C::V;
     constexpr int N = Chunk<E>::N;
     constexpr int ROWS = 64 / LPR;
     const int lane = threadIdx.x & 63;
@@ -129,9 +186,9 @@ __global__ __launch_bounds__(256) void paged_bounds_kernel(BoundsParams p) {
         for (int c0 = 0; c0 < chunks; c0 += LPR) {
             const int c = c0 + (lane & (LPR - 1));
             const E* col = src + min(c, chunks - 1) * N;
-            float lo[N], hi[N];  // smallest values, and smallest negated ones
+            V lo[C::N], hi[C::N];  // smallest values, and smallest negated ones
 #pragma unroll
-            for (int i = 0; i < N; ++i) lo[i] = hi[i] = __builtin_inff();
+            for (int i = 0; i < C::N; ++i) lo[i] = hi[i] = C::largest();
             for (int r0 = 0; r0 < n; r0 += kAhead * ROWS) {
                 u32x4 w[kAhead];
 #pragma unroll
@@ -139,37 +196,45 @@ __global__ __launch_bounds__(256) void paged_bounds_kernel(BoundsParams p) {
                     w[a] = load16(col + min(r0 + a * ROWS + row0, n - 1) * p.ks[2]);
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a) {
-                    const Chunk<E> x = widen<E>(w[a]);
+                    V x[C::N];
+                    C::read(w[a], x);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        lo[i] = min_nan(lo[i], x.f[i]);
-                        hi[i] = min_nan(hi[i], -x.f[i]);
+                    for (int i = 0; i < C::N; ++i) {
+                        lo[i] = C::smaller_of(lo[i], x[i]);
+                        hi[i] = C::smaller_of(hi[i], -x[i]);
                     }
                 }
             }
-            Chunk<E> out;
+            V out[C::N];
+            auto both = [&](int i, auto other) {
+                lo[i] = C::smaller_of(lo[i], other(lo[i]));
+                hi[i] = C::smaller_of(hi[i], other(hi[i]));
+            };
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if constexpr (LPR <= 1) lo[i] = min_nan(lo[i], dpp_mov<0xB1>(lo[i])), hi[i] = min_nan(hi[i], dpp_mov<0xB1>(hi[i]));
-                if constexpr (LPR <= 2) lo[i] = min_nan(lo[i], dpp_mov<0x4E>(lo[i])), hi[i] = min_nan(hi[i], dpp_mov<0x4E>(hi[i]));
-                if constexpr (LPR <= 4) lo[i] = min_nan(lo[i], dpp_mov<0x124>(lo[i])), hi[i] = min_nan(hi[i], dpp_mov<0x124>(hi[i]));
-                if constexpr (LPR <= 8) lo[i] = min_nan(lo[i], dpp_mov<0x128>(lo[i])), hi[i] = min_nan(hi[i], dpp_mov<0x128>(hi[i]));
-                if constexpr (LPR <= 16) lo[i] = min_of_rows<16>(lo[i], lo[i]), hi[i] = min_of_rows<16>(hi[i], hi[i]);
+            for (int i = 0; i < C::N; ++i) {
+                if constexpr (LPR <= 1) both(i, [](V v) { return C::template moved<0xB1>(v); });
+                if constexpr (LPR <= 2) both(i, [](V v) { return C::template moved<0x4E>(v); });
+                if constexpr (LPR <= 4) both(i, [](V v) { return C::template moved<0x124>(v); });
+                if constexpr (LPR <= 8) both(i, [](V v) { return C::template moved<0x128>(v); });
+                if constexpr (LPR <= 16) {
+                    lo[i] = C::template over_rows<16>(lo[i], lo[i]);
+                    hi[i] = C::template over_rows<16>(hi[i], hi[i]);
+                }
                 if constexpr (LPR <= 32) {
-                    out.f[i] = min_of_rows<32>(lo[i], hi[i]);
-                    if (lane >= 32) out.f[i] = -out.f[i];
+                    out[i] = C::template over_rows<32>(lo[i], hi[i]);
+                    if (lane >= 32) out[i] = -out[i];
                 } else {
-                    out.f[i] = lo[i];
+                    out[i] = lo[i];
                 }
             }
             if (c >= chunks) continue;
             if constexpr (LPR <= 32) {
-                if ((lane & 31) < LPR) *reinterpret_cast<u32x4*>(dst + (lane >= 32 ? p.D : 0) + c * N) = narrow<E>(out);
+                if ((lane & 31) < LPR) *reinterpret_cast<u32x4*>(dst + (lane >= 32 ? p.D : 0) + c * N) = C::write(out);
             } else {
-                *reinterpret_cast<u32x4*>(dst + c * N) = narrow<E>(out);
+                *reinterpret_cast<u32x4*>(dst + c * N) = C::write(out);
 #pragma unroll
-                for (int i = 0; i < N; ++i) out.f[i] = -hi[i];
-                *reinterpret_cast<u32x4*>(dst + p.D + c * N) = narrow<E>(out);
+                for (int i = 0; i < C::N; ++i) out[i] = -hi[i];
+                *reinterpret_cast<u32x4*>(dst + p.D + c * N) = C::write(out);
             }
         }
     }

@@ -515,9 +515,12 @@ int64_t bwd_blocks(const NormGrid& g) {
 // its tensors are larger than the last-level cache (256 MB), lines that nobody
 // reads again only push others out.  [4,32/32,4096,128] bf16 forward and
 // backward 274 -> 223 us; [2,32/8,1023,128] kernels 31.4 -> 33.9, so smaller
-// ones keep to the caches, where the next operator finds their results.
+// ones keep to the caches, where the next operator finds their results.  Half
+// rows that share a 128-byte line have to keep to them as well, or each line is
+// read twice: [12,32/32,1317,96] 273 us streamed, 241 not.
 bool streams(int64_t rows, int D, int dtype, int tensors) {
-    return rows * D * (dtype == SA_F32 ? 4 : 2) * tensors > (int64_t(256) << 20);
+    const int size = dtype == SA_F32 ? 4 : 2;
+    return D / 2 * size % 128 == 0 && rows * D * size * tensors > (int64_t(256) << 20);
 }
 
 }  // namespace
