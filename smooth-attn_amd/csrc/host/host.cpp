@@ -23,10 +23,13 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/version.h>
@@ -38,6 +41,8 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "smooth_attn_amd.h"
 
@@ -601,6 +606,44 @@ void qk_norm_fwd(const Tensor& q, const Tensor& k, const Tensor* qw, const Tenso
           "sa_qk_norm_rope_fwd");
 }
 
+// A backward that is being captured, and reaches a leaf whose gradient
+// accumulator belongs to an earlier graph that still lives (a leaf has one as long
+// as any graph holds it) and so to another stream: at its end the engine makes the
+// two streams wait for each other, which a capture cannot hold, and the process
+// ends.  Raised here instead, before that; called from a node's backward.
+void refuse_foreign_leaves(c10::Device device) {
+    const auto current = c10::hip::getCurrentHIPStream(device.index());
+    {
+        const c10::DeviceGuard guard(device);
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    }
+    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
+    if (!node) return;
+    std::vector<torch::autograd::Node*> todo{node.get()};
+    std::unordered_set<torch::autograd::Node*> seen{node.get()};
+    while (!todo.empty()) {
+        torch::autograd::Node* n = todo.back();
+        todo.pop_back();
+        if (n->num_outputs() == 0) {  // a leaf's
+            const auto stream = n->stream();
+            TORCH_CHECK(!stream || (stream->id() == current.id() && stream->device_index() == device.index()),
+                        "sp2norm_qk_norm_rope: this backward is being captured into a graph while an earlier autograd "
+                        "graph of the same leaves lives on another stream; drop that graph's outputs first");
+        }
+        for (uint32_t i = 0; i < n->num_outputs(); ++i)
+            if (n->task_should_compute_output(i) && seen.insert(n->next_edge(i).function.get()).second)
+                todo.push_back(n->next_edge(i).function.get());
+    }
+}
+
+// check_capture(x): raises as the native backward does; for the backward of a node of Python's.
+PyObject* py_check_capture(PyObject*, PyObject* x) {
+    HANDLE_TH_ERRORS
+    if (THPVariable_Check(x) && THPVariable_Unpack(x).is_cuda()) refuse_foreign_leaves(THPVariable_Unpack(x).device());
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 struct QKNorm : public torch::autograd::Function<QKNorm> {
     using MaybeTensor = std::optional<Tensor>;
     static const Tensor* get(const MaybeTensor& t) { return t.has_value() ? &*t : nullptr; }
@@ -635,6 +678,9 @@ struct QKNorm : public torch::autograd::Function<QKNorm> {
                                                                    opt[2], &grads[0], &grads[1]})
             TORCH_CHECK_VALUE(t == nullptr || (t->is_cuda() && t->device() == saved[0].device()),
                               "the norm's tensors must live on the same CUDA device as q");
+        // (only the tensors given have an edge)
+        const bool need_w[2] = {opt[0] && ctx->needs_input_grad(2), opt[1] && ctx->needs_input_grad(opt[0] ? 3 : 2)};
+        refuse_foreign_leaves(saved[0].device());
         const Tensor q = fix(saved[0]), k = fix(saved[1]);
         const auto plain_table = [](const Tensor& t) {
             return t.is_contiguous() && aligned16(t) ? t : t.clone(at::MemoryFormat::Contiguous);
@@ -651,9 +697,8 @@ struct QKNorm : public torch::autograd::Function<QKNorm> {
         const Tensor gq = fix(grads[0].to(q.scalar_type())), gk = fix(grads[1].to(q.scalar_type()));
         const int B = dim(q, 0), Hq = dim(q, 1), Hkv = dim(k, 1), T = dim(q, 2), D = dim(q, 3);
         Tensor dq = output_like(q), dk = output_like(k), dw[2], ws;
-        // (only the tensors given have an edge)
-        if (qw && ctx->needs_input_grad(2)) dw[0] = at::empty_like(*qw);
-        if (kw && ctx->needs_input_grad(qw ? 3 : 2)) dw[1] = at::empty_like(*kw);
+        if (need_w[0]) dw[0] = at::empty_like(*qw);
+        if (need_w[1]) dw[1] = at::empty_like(*kw);
         const bool any = dw[0].defined() || dw[1].defined();
         const int64_t ws_bytes = any ? abi.qk_norm_rope_bwd_workspace_size(B, Hq, Hkv, T, D) : 0;
         if (any) ws = at::empty({ws_bytes / 4}, q.options().dtype(at::kFloat));
@@ -1008,6 +1053,7 @@ PyMethodDef methods[] = {
      "paged_append(k_cache, v_cache, k_new, v_new, block_table, context_lens, block_size) -> lens or None"},
     {"qk_norm_rope", fast(py_qk_norm_rope), METH_FASTCALL,
      "qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps) -> (q', k') or None"},
+    {"check_capture", py_check_capture, METH_O, "check_capture(x): in a backward on x's device"},
     {"paged_norm_append", fast(py_paged_norm_append), METH_FASTCALL,
      "paged_norm_append(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, eps, block_size) "
      "-> q' or None"},

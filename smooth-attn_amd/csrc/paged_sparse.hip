@@ -714,7 +714,7 @@ int check_pages(int B, int Hkv, int D, int page_size, int max_pages, int n_pages
     if (!cache_type(cache)) return SA_ERR_BAD_DTYPE;
     if (D < 8 || D > 1024 || D % 8 != 0 || (cache == SA_FP8_E4M3FN && D % 16 != 0)) return SA_ERR_UNSUPPORTED;
     if (static_cast<int64_t>(max_pages) * page_size > INT32_MAX / 2 ||
-        static_cast<int64_t>(B) * Hkv > INT32_MAX / 64)
+        static_cast<int64_t>(B) * Hkv > INT32_MAX / 1024)  // (the choice's blocks of up to 1024 threads: below 2^32)
         return SA_ERR_UNSUPPORTED;
     return bt_stride < max_pages ? SA_ERR_BAD_STRIDE : 0;
 }

@@ -157,7 +157,7 @@ class NothingOrdinary:
         return None
 
     norm_out = causal_norm = flash = paged = paged_append = _none
-    qk_norm_rope = paged_norm_append = paged_reserve = paged_release = _none
+    qk_norm_rope = check_capture = paged_norm_append = paged_reserve = paged_release = _none
     paged_key_bounds = paged_select_pages = paged_sparse = _none
 
 

@@ -39,10 +39,18 @@ def _check_norm_args(names, tensors, weights, cos, sin, D):
         raise ValueError("cos and sin have no gradient: pass them detached")
 
 
+_INT_DTYPES = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+# Tokens of one launch (heads and head dims past them make up the rest of 2^32 threads).
+MAX_NORM_TOKENS = 1 << 24
+
+
 def _int32(name, t):
-    """A 32-bit copy or view of an integer tensor."""
-    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+    """A contiguous 32-bit copy or view of an integer tensor; 64-bit values past
+    32 bits become the nearest that fit, so none is taken for another."""
+    if t.dtype not in _INT_DTYPES:
         raise ValueError(f"{name} must be an integer tensor, got {t.dtype}")
+    if t.dtype == torch.int64:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
     return t.to(torch.int32).contiguous()
 
 
@@ -96,8 +104,8 @@ def _qk_norm_rope_bwd(q, k, gq, gk, q_weight, k_weight, cos, sin, positions, eps
     Hkv = k.shape[1]
     # (saved-tensor hooks may hand back other types, sizes or layouts)
     _check_norm_args(("q", "k"), (q, k), (q_weight, k_weight), cos.detach(), sin.detach(), D)
-    if (k.shape != (B, Hkv, T, D) or gq.shape != q.shape or gk.shape != k.shape
-            or (positions is not None and positions.dtype != torch.int32)):
+    if (k.shape != (B, Hkv, T, D) or gq.shape != q.shape or gk.shape != k.shape or cos.shape[0] == 0 < B * T
+            or (positions is not None and (positions.dtype != torch.int32 or positions.shape not in ((T,), (B, T))))):
         raise ValueError("the saved tensors of the norm must have the shapes and types that forward saved")
     dq, dk = _output_like(q), _output_like(k)
     dqw = torch.empty_like(q_weight) if need_qw else None
@@ -141,6 +149,7 @@ class _QKNormRopeFn(torch.autograd.Function):
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         need = ctx.needs_input_grad
+        _native().check_capture(q)
         dq, dk, dqw, dkw = _qk_norm_rope_bwd(q, k, gq, gk, q_weight, k_weight, cos, sin, positions, ctx.eps,
                                              need[2], need[3])
         return dq if need[0] else None, dk if need[1] else None, dqw, dkw, None, None, None, None
@@ -159,7 +168,11 @@ def sp2norm_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, 
 
     ``z = x * rsqrt(mean(x^2) + eps) * weight``, then the pair (d, d + D/2) of z
     is turned by its angle; fp32 inside, rounded once.  Returns (q', k') for
-    ``sp2norm_flash_attention``."""
+    ``sp2norm_flash_attention``.
+
+    Forward and ``torch.autograd.grad`` can be captured in a HIP graph; while
+    another autograd graph of the same leaves lives, the captured backward
+    raises RuntimeError."""
     y = _native().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)
     if y is not None:
         return y
@@ -170,6 +183,8 @@ def sp2norm_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, 
     if k.shape[0] != B or k.shape[2] != T or k.shape[3] != D:
         raise ValueError(f"k must be [{B}, H_kv, {T}, {D}], got {tuple(k.shape)}")
     _check_norm_args(("q", "k"), (q, k), (q_weight, k_weight), cos, sin, D)
+    if B * T > MAX_NORM_TOKENS:
+        raise ValueError(f"the norm takes at most {MAX_NORM_TOKENS} tokens, got {B} x {T}")
     if positions is None:
         if cos.shape[0] < T:
             raise ValueError(f"cos and sin must have a row for each of the {T} tokens, got {cos.shape[0]}")

@@ -23,7 +23,7 @@ import torch
 from . import _lib
 from .kernels import (_CACHE_CODE, _DTYPE_CODE, _PAGED_CACHE_DTYPES, _check_paging_args, _check_same_device,
                       _device_of, _flash_operand, _native, _paged_dtype_code, _rope_tables, _stream)
-from .qk_norm import _check_norm_args, _check_tensors, _int32, _norm_weights, _output_like
+from .qk_norm import MAX_NORM_TOKENS, _check_norm_args, _check_tensors, _int32, _norm_weights, _output_like
 
 __all__ = ["PagedReservation", "sp2norm_paged_key_bounds", "sp2norm_paged_qk_norm_rope_append",
            "sp2norm_paged_release", "sp2norm_paged_reserve", "sp2norm_paged_select_pages",
@@ -180,6 +180,8 @@ def sp2norm_paged_qk_norm_rope_append(q, k, v, q_weight, k_weight, cos, sin, pos
     Hkv = k.shape[1]
     with torch.no_grad():
         _check_norm_args(("q", "k", "v"), (q, k, v), (q_weight, k_weight), cos, sin, D)
+        if N > MAX_NORM_TOKENS:
+            raise ValueError(f"the norm takes at most {MAX_NORM_TOKENS} tokens, got {N}")
         _check_caches(block_size, k_cache=k_cache, v_cache=v_cache)
         if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or k_cache.shape[1] != Hkv \
                 or k_cache.shape[3] != D:

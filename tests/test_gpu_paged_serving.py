@@ -141,6 +141,20 @@ def test_append_of_nothing_and_into_strided_caches():
     assert none.shape == (0, 4, D) and torch.equal(k2, kc)
 
 
+def test_64_bit_slots_and_positions_past_32_bits():
+    D = 32
+    cos, sin = smooth_attn.precompute_rope_cos_sin(D, 8, device=DEV)
+    k = _randn((4, 2, D), BF, 1).to(DEV)
+    kc, vc = (torch.zeros(2, 2, 16, D, dtype=BF, device=DEV) for _ in range(2))
+    slots = torch.tensor([1 << 32, 3, -(1 << 32), (1 << 32) + 5], device=DEV)  # 0, 3, 0 and 5 in their low halves
+    pos = torch.tensor([0, (1 << 32) + 1, 2, 3], device=DEV)                   # 1 in its low half; clamped to 7
+    out = smooth_attn.sp2norm_paged_qk_norm_rope_append(k, k, k, None, None, cos, sin, pos, slots, kc, vc)
+    assert torch.equal(vc[0, :, 3], k[1]) and int((vc != 0).any(-1).sum()) == 2
+    want = smooth_attn.sp2norm_qk_norm_rope(k.transpose(0, 1)[None], k.transpose(0, 1)[None], None, None, cos, sin,
+                                            positions=torch.tensor([0, 7, 2, 3], device=DEV))[0]
+    assert torch.equal(out, want[0].transpose(0, 1))
+
+
 def test_append_without_pages_or_query_heads():
     D = 32
     cos, sin = torch.ones(8, 16, device=DEV), torch.zeros(8, 16, device=DEV)

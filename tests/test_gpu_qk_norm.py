@@ -345,3 +345,40 @@ def test_tensors_past_the_caches(dtype, B, T):
         assert all(torch.equal(whole[i][b:b + 1], parts[b][i]) for b in range(B)), i
     for i in (4, 5):  # sums of 32-bit terms in another order
         torch.testing.assert_close(whole[i], sum(p[i] for p in parts), rtol=1e-4, atol=1e-2)
+
+
+@pytest.mark.parametrize("leaf", ["itself", "behind views"])
+@pytest.mark.parametrize("native", [True, False])
+def test_capture_beside_a_living_graph_of_the_same_leaves_is_refused(native, leaf):
+    # (the streams of the two graphs would wait for each other inside the capture, which ends the process)
+    D, T = 64, 20
+    q = _randn((1, 4, T, D), torch.bfloat16, 1).to(DEV)
+    if not native:
+        q = q.transpose(2, 3).contiguous().transpose(2, 3)  # a layout that the Python path takes
+    q.requires_grad_(True)
+    k = _randn((1, 2, T, D), torch.bfloat16, 2).to(DEV)
+    cos, sin = (t.to(DEV) for t in _tables(T, D))
+    ones = torch.ones(q.shape, dtype=q.dtype, device=DEV)
+
+    def forward():
+        x = q if leaf == "itself" else (q * 1).view_as(q)
+        return smooth_attn.sp2norm_qk_norm_rope(x, k, None, None, cos, sin)
+
+    def step():
+        return torch.autograd.grad(forward()[0], q, ones)[0]
+
+    want = step()
+    alive = forward()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="captured into a graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    assert torch.equal(torch.autograd.grad(alive[0], q, ones)[0], want)  # the living graph is as it was
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

@@ -49,6 +49,8 @@ def norm(q=None, k=None, qw=None, kw=None, cos=None, sin=None, **kw_):
     (dict(positions=z(2, 7, dtype=I32)), "positions must be"),
     (dict(positions=z(2, 8, dtype=F32)), "integer"),
     (dict(positions=z(8, dtype=torch.bool)), "integer"),
+    (dict(q=z(1, 1, 1, 16).expand(1 << 13, 1, 1 << 12, 16), k=z(1, 1, 1, 16).expand(1 << 13, 1, 1 << 12, 16),
+          cos=z(1, 8, dtype=F32), sin=z(1, 8, dtype=F32)), "tokens"),
 ])
 def test_norm_refusals(kwargs, match):
     with pytest.raises(ValueError, match=match):
