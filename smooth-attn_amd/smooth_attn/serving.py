@@ -7,8 +7,8 @@ A step over packed new tokens (one each in decode, whole prompts in prefill):
     r = sp2norm_paged_reserve(table, lens, new_lens, free_pages, n_free, n_tokens)
     q = sp2norm_paged_qk_norm_rope_append(q, k, v, q_weight, k_weight, cos, sin, r.positions, r.slots, kc, vc)
     sp2norm_paged_key_bounds(kc, table, lens, r.context_lens, bounds)
-    pages = sp2norm_paged_select_pages(q, bounds, table, r.context_lens, top_k)          # decode
-    o = sp2norm_paged_sparse_attention(q, kc, vc, table, r.context_lens, pages)
+    pages = sp2norm_paged_select_pages(q[:, :, None], bounds, table, r.context_lens, top_k)   # decode
+    o = sp2norm_paged_sparse_attention(q[:, :, None], kc, vc, table, r.context_lens, pages)
 
 The caches and tables are plain tensors of the caller's; none of these calls
 has a gradient (like the paged attention).
