@@ -17,7 +17,9 @@
 // One launch: every block works out the sums for itself (they are a few
 // thousand numbers), and a new page's first token, whose thread knows the page
 // anyway, enters it into the table.  The entries that are read (below had_b)
-// are never the ones that are written.
+// are never the ones that are written.  Bound by the launch and a chain of loads
+// and sums: 3.6 us for a token of each of 64 sequences, 5.7 for 67600 tokens of
+// 256.
 #include "common.hpp"
 
 namespace sa {

@@ -155,7 +155,10 @@ struct BoundsParams {
 // row (or 64 chunks of it at a time) and 64 / LPR rows are read at once, kAhead
 // such reads before the first is used.  Largest values are kept as smallest
 // negated ones, so both are the same operation: at the last exchange the lower
-// half of the wave takes over the one kind and the upper half the other.
+// half of the wave takes over the one kind and the upper half the other.  Four
+// prompts of 8192 to 16384 tokens, Hkv 8, D = 128 bf16: 26 us, 4.4 TB/s (37 us with
+// both kinds exchanged over LDS and one page's loads behind another's); e4m3fn
+// keys take 1.7 times their bytes, for unpacking.
 constexpr int kAhead = 4;
 template <typename E, int LPR>
 __global__ __launch_bounds__(256) void paged_bounds_kernel(BoundsParams p) {
@@ -340,7 +343,9 @@ __device__ __forceinline__ int first_value() {
 // chunks first); the lane's parts of Q- and Q+ stay in registers, in 64 bits.  A
 // wave takes kBatch loads' pages at a time: their table entries are read a batch
 // ahead, their bounds all before the first is used, and their sums are added up
-// together.
+// together.  Bound by memory, 512 bytes a page and KV head anywhere in it: 138 MB
+// (64 sequences of 512 to 16384 tokens) 35 us, 201 MB (8 of 65536 to 131072) 42;
+// with one load in flight and each sum exchanged alone 83 and 88.
 constexpr int kBatch = 8;
 template <typename E, int LPP, int NCH>
 __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
