@@ -579,8 +579,9 @@ int sa_paged_release(int32_t* block_table, const int32_t* context_lens,
  * page's tokens (NaN where one is), for the pages that hold tokens from_lens[b]
  * .. to_lens[b] - 1 of each sequence; a page's tokens from its first on up to
  * to_lens[b] count, also those before from_lens[b].  Table entries that name no
- * page are skipped.  Page sizes, head dims (8..1024) and cache types as
- * sa_paged_decode; max_pages * page_size < 2^30.
+ * page are skipped; a page that two sequences share must be full in both.  Page
+ * sizes, head dims (8..1024) and cache types as sa_paged_decode; max_pages *
+ * page_size < 2^30, B * Hkv < 2^21.
  */
 int sa_paged_key_bounds(const void* k_cache, void* bounds,
                         const int32_t* block_table, const int32_t* from_lens,
@@ -598,9 +599,11 @@ int sa_paged_key_bounds(const void* k_cache, void* bounds,
  *   score = sum_d Q+_d bounds[page, h, 1, d] + Q-_d bounds[page, h, 0, d],
  * Q+ / Q- = sum over the KV head's query heads of max(q, 0) / min(q, 0), in 64
  * bits; equal scores: the lower page; NaN above all.  n_first + n_last <=
- * top_k.  q [B, Hq, 1, D] of dtype SA_BF16 / SA_F16 / SA_F32 with unit d
- * stride; bounds of cache_dtype (sa_paged_key_bounds).  workspace (8-byte
- * aligned): sa_paged_select_workspace_size() bytes where top_k < max_pages.
+ * top_k.  Table entries outside [0, n_pages) are clamped.  q [B, Hq, 1, D] of
+ * dtype SA_BF16 / SA_F16 / SA_F32, 16-byte aligned, unit d stride, the others
+ * multiples of 16 bytes; bounds of cache_dtype (sa_paged_key_bounds), 16-byte
+ * aligned.  B * Hkv < 2^21.  workspace (8-byte aligned):
+ * sa_paged_select_workspace_size() bytes where top_k < max_pages.
  */
 int64_t sa_paged_select_workspace_size(int B, int Hkv, int max_pages);
 int sa_paged_select_pages(const void* q, const void* bounds,

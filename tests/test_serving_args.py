@@ -255,9 +255,12 @@ def test_append_bounds_select_sparse_abi_errors():
     assert bnd(cache=5) == -3 and bnd(stride=3) == -5 and bnd(k=None) == -1 and bnd(k=BAD) == -5
     assert bnd(W=1 << 27, stride=1 << 27) == -6 and bnd(cache=_lib.SA_FP8_E4M3FN, D=24) == -6
 
-    def sel(B=2, Hq=4, K=2, first=0, last=1, W=4, ws=D16, nbytes=1 << 40, dt=_lib.SA_BF16, pages=D16):
-        return lib.sa_paged_select_pages(D16, D16, D16, D16, pages, B, Hq, 2, 64, 16, W, 8, K, first, last, t4, W, dt,
+    def sel(B=2, Hq=4, K=2, first=0, last=1, W=4, ws=D16, nbytes=1 << 40, dt=_lib.SA_BF16, pages=D16, q=D16, s=t4):
+        return lib.sa_paged_select_pages(q, D16, D16, D16, pages, B, Hq, 2, 64, 16, W, 8, K, first, last, s, W, dt,
                                          _lib.SA_BF16, ws, nbytes, None)
+
+    assert sel(q=BAD) == -5 and sel(s=_s(2048, 60, 64, 1)) == -5 and sel(s=_s(2048, 64, 64, 2)) == -5
+    assert sel(B=1 << 21) == -6
 
     assert sel(B=0) == 0 and sel(K=0, last=0) == 0 and sel(Hq=3) == -2 and sel(K=-1) == -2 and sel(first=2) == -2
     assert sel(last=-1) == -2 and sel(dt=3) == -3 and sel(pages=None) == -1 and sel(nbytes=8) == -7 and sel(ws=None) == -7
