@@ -564,7 +564,9 @@ int sa_paged_reserve(int32_t* block_table, const int32_t* context_lens,
  * The pages of the sequences whose finished[b] is not 0 go back on the stack,
  * in the order of the sequences and their tables; their table entries become
  * -1 (entries that name no page are skipped) and lens_out[b] 0, that of the
- * others context_lens[b].  counts_ws: int32 [B] of workspace.  B >= 1.
+ * others context_lens[b].  A page is pushed as often as a finished sequence's
+ * table names it: set the entries of pages that others still read to -1 first.
+ * counts_ws: int32 [B] of workspace.  B >= 1.
  */
 int sa_paged_release(int32_t* block_table, const int32_t* context_lens,
                      const uint8_t* finished, int32_t* free_pages,

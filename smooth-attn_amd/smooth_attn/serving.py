@@ -114,8 +114,10 @@ def sp2norm_paged_reserve(block_table, context_lens, new_lens, free_pages, n_fre
 def sp2norm_paged_release(block_table, context_lens, finished, free_pages, n_free, *, block_size=16):
     """Give the pages of finished sequences (bool [B]) back: they are pushed on
     the stack free_pages in place, in the order of the sequences and their
-    tables, and their table entries become -1.  Returns (context_lens, n_free):
-    lengths with 0 for the finished ones, and the new number of free pages."""
+    tables, and their table entries become -1.  A page goes on the stack as often
+    as a finished sequence's table names it: one that other sequences still read
+    has to leave the table (-1) first.  Returns (context_lens, n_free): lengths
+    with 0 for the finished ones, and the new number of free pages."""
     out = _native().paged_release(block_table, context_lens, finished, free_pages, n_free, block_size)
     if out is not None:
         return out
