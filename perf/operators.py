@@ -26,9 +26,6 @@ import sys
 
 import torch
 
-# where the package lies (imported only where own is true)
-sys.path.insert(1, str(pathlib.Path(__file__).resolve().parent.parent / "smooth-attn_amd"))
-
 own = False
 
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32, "fp8": torch.float8_e4m3fn}
@@ -405,6 +402,14 @@ def _plain_sparse(s, pages):
 # ---------------------------------------------------------------------------
 # One pass.
 # ---------------------------------------------------------------------------
+def _package():
+    path = str(pathlib.Path(__file__).resolve().parent.parent / "smooth-attn_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import smooth_attn
+    return smooth_attn
+
+
 def _maps(s, release, reserve):
     """The tables of a step (of copies, where the pass changes what it starts from)."""
     table, lens, free, n_free = s["table"], s["lens"], s["free"], s["n_free"]
@@ -419,7 +424,7 @@ def run(s):
     case = s["case"]
     kind = case["kind"]
     if own:
-        import smooth_attn as sa
+        sa = _package()
         if kind == "norm_rope":
             q, k = sa.sp2norm_qk_norm_rope(s["q"], s["k"], s["qw"], s["kw"], s["cos"], s["sin"], eps=NORM_EPS)
             if not case["grad"]:
