@@ -621,7 +621,8 @@ int sa_paged_select_pages(const void* q, const void* bounds,
  * sa_paged_decode over listed pages only: pages [B, Hkv, n_listed] (contiguous
  * int32) holds indexes into the sequence's table row, in any order; those
  * outside [0, max_pages) are skipped, and of a page the tokens below
- * context_lens[b] count, once for every time it is listed.  Everything else as
+ * context_lens[b] count, once for every time it is listed.  With SA_F16 alone,
+ * weights are finite for scores (scale q . k) up to 1023.  Everything else as
  * sa_paged_decode; workspace: sa_paged_sparse_workspace_size() bytes, 16-byte
  * aligned, contents ignored.
  */

@@ -262,6 +262,7 @@ __global__ __launch_bounds__(64 * WPB) void paged_partial_kernel(PagedParams p) 
     constexpr int TPI = 64 / CPT;          // tokens per load instruction
     constexpr int NC = kTile * CPT / 64;   // chunks per lane per tile and tensor
     constexpr bool SQ = Ty::SPLIT_Q, SC = Ty::SPLIT_C, SP = Ty::SPLIT_P;
+    constexpr bool IN_PASSES = Plan::LISTED && std::is_same_v<T, f16>;
     // MT tiles (one set per wave); the lo parts of split caches in the second pair
     __shared__ __attribute__((aligned(16))) T ldsK_w[WPB][kTile * RS];
     __shared__ __attribute__((aligned(16))) T ldsV_w[WPB][kTile * RSV];
@@ -498,36 +499,65 @@ __global__ __launch_bounds__(64 * WPB) void paged_partial_kernel(PagedParams p) 
                     y[v] = (Plan::LISTED ? (tokens >> r) & 1 : t0 + r < we) ? wgt : 0.f;
                     ssum += y[v];
                 }
+                // fp16 weights end at 65504, that of a score of 128.  A tile with a
+                // larger one is added in passes of up to 65504 each (what a pass
+                // leaves is exact), 64 at most; past their sum, a score of 1023,
+                // the weight is infinite.
+                int passes = 1;
+                float rest[IN_PASSES ? 16 : 1];
+                auto next_pass = [&]() {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t ph[4], plo[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if constexpr (SP)
-                            split2_bf16(y[8 * c + 2 * j], y[8 * c + 2 * j + 1], ph[j], plo[j]);
-                        else
-                            ph[j] = pack2<T>(y[8 * c + 2 * j], y[8 * c + 2 * j + 1]);
+                    for (int v = 0; v < 16; ++v) {
+                        y[v] = passes > 1 ? __builtin_fminf(rest[v], 65504.f) : rest[v];
+                        rest[v] -= y[v];
                     }
-                    const u32x4 pw{ph[0], ph[1], ph[2], ph[3]};
-                    const u32x4 pl = SP ? u32x4{plo[0], plo[1], plo[2], plo[3]} : u32x4{0u, 0u, 0u, 0u};
-                    const Vec bop = as_vec8<Vec>(pw);
+                };
+                if constexpr (IN_PASSES) {
+                    float most = y[0];
 #pragma unroll
-                    for (int dt = 0; dt < D / 32; ++dt) {
-                        const T* base = ldsV + (16 * c) * RSV + dt * 32 + v_tr_off;
-                        const uint2 lo = lds_read_tr16(base);
-                        const uint2 hi8 = lds_read_tr16(base + 8 * RSV);
-                        const u32x4 aw{lo.x, lo.y, hi8.x, hi8.y};
-                        oacc[dt] = Ops::mma(as_vec8<Vec>(aw), bop, oacc[dt]);
-                        if constexpr (SP) oacc[dt] = Ops::mma(as_vec8<Vec>(aw), as_vec8<Vec>(pl), oacc[dt]);
-                        if constexpr (SC) {
-                            const T* basel = ldsVl + (16 * c) * RSV + dt * 32 + v_tr_off;
-                            const uint2 lol = lds_read_tr16(basel);
-                            const uint2 hil = lds_read_tr16(basel + 8 * RSV);
-                            const u32x4 awl{lol.x, lol.y, hil.x, hil.y};
-                            oacc[dt] = Ops::mma(as_vec8<Vec>(awl), bop, oacc[dt]);
-                        }
+                    for (int v = 1; v < 16; ++v) most = __builtin_fmaxf(most, y[v]);
+                    if (__ballot(most > 65504.f) != 0) {
+                        passes += static_cast<int>(__builtin_fminf(wave_max(most) * (1.f / 65504.f), 63.f));
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) rest[v] = y[v];
+                        next_pass();
                     }
                 }
+                do {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t ph[4], plo[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if constexpr (SP)
+                                split2_bf16(y[8 * c + 2 * j], y[8 * c + 2 * j + 1], ph[j], plo[j]);
+                            else
+                                ph[j] = pack2<T>(y[8 * c + 2 * j], y[8 * c + 2 * j + 1]);
+                        }
+                        const u32x4 pw{ph[0], ph[1], ph[2], ph[3]};
+                        const u32x4 pl = SP ? u32x4{plo[0], plo[1], plo[2], plo[3]} : u32x4{0u, 0u, 0u, 0u};
+                        const Vec bop = as_vec8<Vec>(pw);
+#pragma unroll
+                        for (int dt = 0; dt < D / 32; ++dt) {
+                            const T* base = ldsV + (16 * c) * RSV + dt * 32 + v_tr_off;
+                            const uint2 lo = lds_read_tr16(base);
+                            const uint2 hi8 = lds_read_tr16(base + 8 * RSV);
+                            const u32x4 aw{lo.x, lo.y, hi8.x, hi8.y};
+                            oacc[dt] = Ops::mma(as_vec8<Vec>(aw), bop, oacc[dt]);
+                            if constexpr (SP) oacc[dt] = Ops::mma(as_vec8<Vec>(aw), as_vec8<Vec>(pl), oacc[dt]);
+                            if constexpr (SC) {
+                                const T* basel = ldsVl + (16 * c) * RSV + dt * 32 + v_tr_off;
+                                const uint2 lol = lds_read_tr16(basel);
+                                const uint2 hil = lds_read_tr16(basel + 8 * RSV);
+                                const u32x4 awl{lol.x, lol.y, hil.x, hil.y};
+                                oacc[dt] = Ops::mma(as_vec8<Vec>(awl), bop, oacc[dt]);
+                            }
+                        }
+                    }
+                    if constexpr (IN_PASSES) {
+                        if (--passes > 0) next_pass();
+                    }
+                } while (IN_PASSES && passes > 0);
                 __builtin_amdgcn_wave_barrier();
             }
             ws = we;

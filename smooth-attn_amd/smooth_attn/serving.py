@@ -340,7 +340,8 @@ def sp2norm_paged_sparse_attention(q, k_cache, v_cache, block_table, context_len
     KV head (sp2norm_paged_select_pages), in any order; indexes outside the
     table are skipped, of a page the tokens below context_lens[b] count, and a
     page that is listed twice counts twice.  No token at all gives zeros.  The
-    other arguments, types and head dims are sp2norm_paged_attention's."""
+    other arguments, types and head dims are sp2norm_paged_attention's.  Scores
+    (scale q . k) may reach 1023 where q and the caches are fp16."""
     out = _native().paged_sparse(q, k_cache, v_cache, block_table, context_lens, pages, scale, block_size)
     if out is not None:
         return out
