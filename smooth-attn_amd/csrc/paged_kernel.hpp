@@ -775,8 +775,8 @@ int validate_paged(const void* q, const void* k_cache, const void* v_cache, cons
     const int64_t max_ctx = static_cast<int64_t>(max_pages) * page_size;
     if (max_ctx > INT32_MAX / 2 || static_cast<int64_t>(B) * Hkv * ((max_ctx + kTile - 1) / kTile) > INT32_MAX / 2)
         return SA_ERR_UNSUPPORTED;
-    if (!q || !k_cache || !v_cache || !out || !block_table || !context_lens || !q_strides || !kv_strides ||
-        !vv_strides || !o_strides)
+    if (!q || !out || !context_lens || !q_strides || !kv_strides || !vv_strides || !o_strides ||
+        (n_pages > 0 && (!k_cache || !v_cache)) || (max_pages > 0 && !block_table))
         return SA_ERR_NULL_POINTER;
     int qt, ct;
     if (!paged_types(dtype, qt, ct)) return SA_ERR_BAD_DTYPE;

@@ -829,7 +829,7 @@ extern "C" int sa_paged_select_pages(const void* q, const void* bounds, const in
         return SA_ERR_BAD_SHAPE;
     if (dtype != SA_F32 && dtype != SA_F16 && dtype != SA_BF16) return SA_ERR_BAD_DTYPE;
     if (B == 0 || top_k == 0) return 0;
-    if (!q || !pages || !q_strides || !context_lens || (max_pages > 0 && (!bounds || !block_table)))
+    if (!q || !pages || !q_strides || !context_lens || (n_pages > 0 && max_pages > 0 && (!bounds || !block_table)))
         return SA_ERR_NULL_POINTER;
     const int q16 = dtype == SA_F32 ? 4 : 8;
     if (q_strides[3] != 1 || q_strides[0] % q16 != 0 || q_strides[1] % q16 != 0 || !aligned16(q) || !aligned16(bounds) || D % (16 / bytes_of(cache_dtype)) != 0) return SA_ERR_BAD_STRIDE;
