@@ -103,9 +103,9 @@ __device__ __forceinline__ void store8(T* p, const float* f) {
     }
 }
 
-// x rounded to an e4m3fn code: nearest, ties to even, NaN from 464 up as
-// torch's conversion has it (464 is halfway from 448 to the first value past
-// the type).
+// x rounded to an e4m3fn code: nearest, ties to even, NaN past 464 as torch's
+// conversion has it (464 is halfway from 448 to the first value past the type,
+// and goes to 448).
 __device__ __forceinline__ uint32_t e4m3_pair(float a, float b, uint32_t old, bool high) {
     return high ? __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, true) : __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, false);
 }
@@ -128,6 +128,14 @@ __device__ __forceinline__ void store8_cache(void* base, int64_t off, int code, 
     else if (code == SA_F16) store8<f16>(static_cast<f16*>(base) + off, f);
     else if (code == SA_F32) store8<float>(static_cast<float*>(base) + off, f);
     else store8_e4m3(static_cast<uint8_t*>(base) + off, f);
+}
+
+// 1 / sqrt(x), off by 3/4 of a step at most (v_rsq_f32, which takes arguments below
+// the normal range for zero: those are scaled, exactly, on both sides of it).
+__device__ __forceinline__ float rsqrt_of(float x) {
+    const bool small = x < 0x1p-126f;
+    const float r = fast_rsqrt(small ? x * 0x1p32f : x);
+    return small ? r * 0x1p16f : r;
 }
 
 // Sum over the L lanes of a row, in each of them.
@@ -226,7 +234,7 @@ __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_kernel(NormParams 
             float sq = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) sq = __builtin_fmaf(a[i], a[i], __builtin_fmaf(e[i], e[i], sq));
-            const float r = fast_rsqrt(__builtin_fmaf(row_sum<L>(sq), inv_d, p.eps));
+            const float r = rsqrt_of(__builtin_fmaf(row_sum<L>(sq), inv_d, p.eps));
             if (at.live) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -303,7 +311,7 @@ __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_bwd_kernel(NormPar
                         hx = __builtin_fmaf(zl * wl[i], a[i], __builtin_fmaf(zh * wh[i], e[i], hx));
                     }
                 }
-                const float r = fast_rsqrt(__builtin_fmaf(row_sum<L>(sq), inv_d, p.eps));
+                const float r = rsqrt_of(__builtin_fmaf(row_sum<L>(sq), inv_d, p.eps));
                 const float mr = row_sum<L>(hx) * inv_d * r * r;
                 if (at.live) {
                     float xa[8], xe[8];
