@@ -356,8 +356,9 @@ __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_bwd_kernel(NormPar
     }
 }
 
-// dw[d] = sum of n partial rows, in a fixed order: 16 columns a block, 16 lanes
-// of rows for each (4.8 us for 1366 rows of 128).
+// dw[d] = sum of n partial rows, in a fixed order and in 64 bits (the sums over a
+// block's rows are what 32 bits round): 16 columns a block, 16 lanes of rows for
+// each (4.8 us for 1366 rows of 128).
 struct DwParams {
     const float* partial[2];
     void* out[2];
@@ -365,14 +366,14 @@ struct DwParams {
     int D, code;
 };
 __global__ __launch_bounds__(256) void norm_dw_kernel(DwParams p) {
-    __shared__ float red[16][17];
+    __shared__ double red[16][17];
     const int col = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     const int d = blockIdx.x * 16 + col;
     const float* src = p.partial[blockIdx.y] + d;
     const int n = p.n[blockIdx.y];
-    float v = 0.f;
+    double v = 0.0;
 #pragma unroll 8
-    for (int r = r0; r < n; r += 16) v += src[static_cast<int64_t>(r) * p.D];
+    for (int r = r0; r < n; r += 16) v += static_cast<double>(src[static_cast<int64_t>(r) * p.D]);
     red[r0][col] = v;
     __syncthreads();
     if (r0 != 0) return;
@@ -380,9 +381,10 @@ __global__ __launch_bounds__(256) void norm_dw_kernel(DwParams p) {
     for (int i = 1; i < 16; ++i) v += red[i][col];
     void* out = p.out[blockIdx.y];
     if (out == nullptr) return;
-    if (p.code == SA_F32) static_cast<float*>(out)[d] = v;
-    else if (p.code == SA_BF16) static_cast<bf16*>(out)[d] = static_cast<bf16>(v);
-    else static_cast<f16*>(out)[d] = static_cast<f16>(v);
+    const float f = static_cast<float>(v);
+    if (p.code == SA_F32) static_cast<float*>(out)[d] = f;
+    else if (p.code == SA_BF16) static_cast<bf16*>(out)[d] = static_cast<bf16>(f);
+    else static_cast<f16*>(out)[d] = static_cast<f16>(f);
 }
 
 // ---------------------------------------------------------------------------

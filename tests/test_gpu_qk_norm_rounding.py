@@ -1,4 +1,4 @@
-"""Roundings of the norm's reciprocal root (GPU)."""
+"""Roundings of the norm's reciprocal root and of its weight gradients (GPU)."""
 import pytest
 import torch
 
@@ -53,3 +53,18 @@ def test_a_row_of_zeros_without_eps_is_as_the_formula_says():
     x = torch.zeros(1, 1, 3, 64, device=DEV)
     y, _ = smooth_attn.sp2norm_qk_norm_rope(x, x, None, None, *_turned_by_nothing(3, 64), eps=0.0)
     assert torch.isnan(y).all()
+
+
+def test_a_weight_gradient_of_one_large_term():
+    # Rows of ones with gradients of ones: every row's term is 1, but one is 2^34.  A block adds its
+    # 128 rows in fp32 and may lose all of them beside the large one; the sum over blocks loses
+    # nothing but its last rounding, 2^-24.
+    T, H, D = 16384, 8, 64
+    q, g = torch.ones(1, H, T, D, device=DEV), torch.ones(1, H, T, D, device=DEV)
+    g[0, 0, 0] = 2.0 ** 34
+    k = torch.ones(1, 1, T, D, device=DEV)
+    w = torch.ones(D, device=DEV, requires_grad=True)
+    y, _ = smooth_attn.sp2norm_qk_norm_rope(q, k, w, None, *_turned_by_nothing(T, D), eps=0.0)
+    dw = torch.autograd.grad(y, w, g)[0].double().cpu()
+    want = 2.0 ** 34 + H * T - 1
+    assert ((dw - want).abs() <= 128 + U * want).all(), (dw - want).abs().max()
