@@ -492,8 +492,9 @@ int sa_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, void* k_out,
 /*
  * Its backward: dq, dk (dtype) from dq_out, dk_out (dtype), and where given
  * the weights' gradients dq_weight, dk_weight [D] (w_dtype), summed in a fixed
- * order, in fp32 over a block's rows and in 64 bits over the blocks.  workspace: sa_qk_norm_rope_bwd_workspace_size() bytes, 16-byte
- * aligned, contents ignored; only read where a weight gradient is asked for.
+ * order, in fp32 over a block's rows and in 64 bits over the blocks.
+ * workspace: sa_qk_norm_rope_bwd_workspace_size() bytes, 16-byte aligned,
+ * contents ignored; only read where a weight gradient is asked for.
  * With no row (B * T or Hq + Hkv 0) nothing is written and asking for a weight
  * gradient is refused.
  */
