@@ -607,12 +607,13 @@ void qk_norm_fwd(const Tensor& q, const Tensor& k, const Tensor* qw, const Tenso
 }
 
 // A backward that is being captured, and reaches a leaf whose gradient
-// accumulator belongs to an earlier graph that still lives (a leaf has one as long
-// as any graph holds it) and so to another stream: at its end the engine makes the
-// two streams wait for each other, which a capture cannot hold, and the process
-// ends.  Raised here instead, before that; called from a node's backward.
-void refuse_foreign_leaves(c10::Device device) {
-    const auto current = c10::hip::getCurrentHIPStream(device.index());
+// accumulator lives on the default stream, because a graph or a hook made outside
+// of any other stream still holds it (a leaf has one as long as anything does): the
+// engine makes the accumulator's stream and the backward's wait for each other,
+// which the default stream cannot do for a capture, and the process ends.  Raised
+// here instead, before that; called from a node's backward.  Any other stream joins
+// the capture with the first wait and is waited for with the second.
+void refuse_default_stream_leaves(c10::Device device) {
     {
         const c10::DeviceGuard guard(device);
         if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
@@ -626,9 +627,10 @@ void refuse_foreign_leaves(c10::Device device) {
         todo.pop_back();
         if (n->num_outputs() == 0) {  // a leaf's
             const auto stream = n->stream();
-            TORCH_CHECK(!stream || (stream->id() == current.id() && stream->device_index() == device.index()),
-                        "sp2norm_qk_norm_rope: this backward is being captured into a graph while an earlier autograd "
-                        "graph of the same leaves lives on another stream; drop that graph's outputs first");
+            TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(stream->device_index()).id(),
+                        "sp2norm_qk_norm_rope: this backward is being captured into a graph while an autograd graph or "
+                        "a hook of the same leaves lives on the default stream; drop that first, or make it on another "
+                        "stream");
         }
         for (uint32_t i = 0; i < n->num_outputs(); ++i)
             if (n->task_should_compute_output(i) && seen.insert(n->next_edge(i).function.get()).second)
@@ -639,7 +641,7 @@ void refuse_foreign_leaves(c10::Device device) {
 // check_capture(x): raises as the native backward does; for the backward of a node of Python's.
 PyObject* py_check_capture(PyObject*, PyObject* x) {
     HANDLE_TH_ERRORS
-    if (THPVariable_Check(x) && THPVariable_Unpack(x).is_cuda()) refuse_foreign_leaves(THPVariable_Unpack(x).device());
+    if (THPVariable_Check(x) && THPVariable_Unpack(x).is_cuda()) refuse_default_stream_leaves(THPVariable_Unpack(x).device());
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -680,7 +682,7 @@ struct QKNorm : public torch::autograd::Function<QKNorm> {
                               "the norm's tensors must live on the same CUDA device as q");
         // (only the tensors given have an edge)
         const bool need_w[2] = {opt[0] && ctx->needs_input_grad(2), opt[1] && ctx->needs_input_grad(opt[0] ? 3 : 2)};
-        refuse_foreign_leaves(saved[0].device());
+        refuse_default_stream_leaves(saved[0].device());
         const Tensor q = fix(saved[0]), k = fix(saved[1]);
         const auto plain_table = [](const Tensor& t) {
             return t.is_contiguous() && aligned16(t) ? t : t.clone(at::MemoryFormat::Contiguous);

@@ -157,8 +157,19 @@ class NothingOrdinary:
         return None
 
     norm_out = causal_norm = flash = paged = paged_append = _none
-    qk_norm_rope = check_capture = paged_norm_append = paged_reserve = paged_release = _none
+    qk_norm_rope = paged_norm_append = paged_reserve = paged_release = _none
     paged_key_bounds = paged_select_pages = paged_sparse = _none
+
+    @staticmethod
+    def check_capture(x):
+        """Refuses what only the extension can tell apart: a captured backward that
+        may reach leaves whose accumulators live on the default stream, which ends
+        the process."""
+        import torch
+
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("sp2norm_qk_norm_rope: its backward is captured into a graph only with the native call "
+                               "path, which is not available")
 
 
 def _load_host(lib):

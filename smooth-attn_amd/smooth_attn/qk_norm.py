@@ -170,9 +170,10 @@ def sp2norm_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, 
     is turned by its angle; fp32 inside, rounded once.  Returns (q', k') for
     ``sp2norm_flash_attention``.
 
-    Forward and ``torch.autograd.grad`` can be captured in a HIP graph; while
-    another autograd graph of the same leaves lives, the captured backward
-    raises RuntimeError."""
+    Forward and backward can be captured in a HIP graph.  While an autograd graph
+    or a hook made on the default stream holds the same leaves, or without the
+    native call path, the captured backward raises RuntimeError; made on another
+    stream they may live."""
     y = _native().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)
     if y is not None:
         return y
