@@ -870,7 +870,10 @@ PyObject* py_paged_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
         const NoGil released;
         const int64_t B = table->size(0);
-        out = int_vectors({n_tokens, n_tokens, n_tokens, B + 1, B, 1}, *table);
+        // (what a program keeps from step to step holds nothing of the tokens' maps)
+        const auto maps = int_vectors({n_tokens, n_tokens, n_tokens}, *table);
+        const auto lengths = int_vectors({B + 1, B, 1}, *table);
+        out = {maps[0], maps[1], maps[2], lengths[0], lengths[1], lengths[2]};
         const c10::DeviceGuard guard(table->device());
         const auto p = [](const Tensor& t) { return t.data_ptr<int32_t>(); };
         check(abi.paged_reserve(p(*table), p(*lens), p(*fresh), p(*free_pages), p(*n_free), p(out[0]), p(out[1]),

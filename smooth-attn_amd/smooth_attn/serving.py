@@ -34,7 +34,8 @@ MAX_RESERVED_SEQS = 4096
 
 
 class PagedReservation(NamedTuple):
-    """What sp2norm_paged_reserve returns; all int32 on the device."""
+    """What sp2norm_paged_reserve returns; all int32 on the device.  The three maps
+    of tokens may share one allocation, and the others another."""
 
     slots: torch.Tensor         # [n_tokens] cache slot of each packed token, -1 for none
     positions: torch.Tensor     # [n_tokens] its position in its sequence
