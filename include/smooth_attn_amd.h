@@ -544,7 +544,10 @@ int sa_paged_qk_norm_rope_append(
  * .. n_free[0]) (n_pages entries of room) and entered into its row of
  * block_table [B, max_pages].  Sequences are served in order; one that finds
  * too few pages, or whose table or the n_tokens packed tokens end, is cut:
- * lens_out[b] is the length that has pages.
+ * lens_out[b] is the length that has pages.  A sequence has the first
+ * ceil(context_lens[b] / page_size) entries of its row; those past them are taken
+ * as empty and overwritten, so pages past a length that was cut have to be put
+ * back on the stack first.
  *   starts [B + 1]: packed position of each sequence's first new token
  *   slots, positions, sequences [n_tokens]: cache slot (page * page_size + row,
  *     -1 for none), position and sequence (-1 past the last) of each token
@@ -562,11 +565,12 @@ int sa_paged_reserve(int32_t* block_table, const int32_t* context_lens,
                      sa_stream_t stream);
 
 /*
- * The pages of the sequences whose finished[b] is not 0 go back on the stack,
- * in the order of the sequences and their tables; their table entries become
- * -1 (entries that name no page are skipped) and lens_out[b] 0, that of the
- * others context_lens[b].  A page is pushed as often as a finished sequence's
- * table names it: set the entries of pages that others still read to -1 first.
+ * The pages that context_lens[b] tokens take of the sequences whose finished[b]
+ * is not 0 go back on the stack, in the order of the sequences and their tables;
+ * their table entries become -1 (entries that name no page are skipped) and
+ * lens_out[b] 0, that of the others context_lens[b].  A page is pushed as often
+ * as a finished sequence's table names it: set the entries of pages that others
+ * still read to -1 first.
  * counts_ws: int32 [B] of workspace.  B >= 1.
  */
 int sa_paged_release(int32_t* block_table, const int32_t* context_lens,

@@ -79,9 +79,15 @@ def sp2norm_paged_reserve(block_table, context_lens, new_lens, free_pages, n_fre
 
     block_table: int32 [B, max_pages], updated in place past the pages that each
     sequence has; context_lens, new_lens: integer [B], tokens that each sequence
-    has and gets (0 for none); free_pages: int32 [n_pages], a stack of free page
-    ids of which the first n_free (int32, one element) count; n_tokens: room of
-    the packed token tensors (an int; tokens past the sum get slot -1).
+    has and gets (0 for none); free_pages: int32 [n_pages], as long as the caches
+    have pages (other ids name none), a stack of free page ids of which the first
+    n_free (int32, one element) count; n_tokens: room of the packed token tensors
+    (an int; tokens past the sum get slot -1).
+
+    A sequence has the first ceil(context_lens[b] / block_size) entries of its
+    table row; those past them are taken as empty and overwritten.  So a length
+    may not be cut below a page border (rejected tokens, say) before the caller
+    has put the pages past it back on the stack: they would be lost to it.
 
     Sequences are served in their order.  One that finds too few pages, or
     reaches the end of its table row or of the packed tokens, is cut: its
@@ -115,9 +121,10 @@ def sp2norm_paged_reserve(block_table, context_lens, new_lens, free_pages, n_fre
 def sp2norm_paged_release(block_table, context_lens, finished, free_pages, n_free, *, block_size=16):
     """Give the pages of finished sequences (bool [B]) back: they are pushed on
     the stack free_pages in place, in the order of the sequences and their
-    tables, and their table entries become -1.  A page goes on the stack as often
-    as a finished sequence's table names it: one that other sequences still read
-    has to leave the table (-1) first.  Returns (context_lens, n_free): lengths
+    tables, and their table entries become -1: the pages of context_lens[b] tokens,
+    not entries past them.  A page goes on the stack as often as a finished
+    sequence's table names it: one that other sequences still read has to leave the
+    table (-1) first.  Returns (context_lens, n_free): lengths
     with 0 for the finished ones, and the new number of free pages."""
     out = _native().paged_release(block_table, context_lens, finished, free_pages, n_free, block_size)
     if out is not None:
@@ -245,7 +252,8 @@ def sp2norm_paged_key_bounds(k_cache, block_table, from_lens, to_lens, bounds=No
     place and returned (None: a new one, of zeros elsewhere); [:, :, 0] holds the
     smallest values, [:, :, 1] the largest, NaN where a key is.  All of a page's
     tokens below to_lens count, so a page that is filled step by step is right
-    after each.  Table entries that name no page are skipped."""
+    after each; one that sequences share must be full in each.  Table entries that
+    name no page are skipped."""
     if _native().paged_key_bounds(k_cache, block_table, from_lens, to_lens, bounds, block_size):
         return bounds
     _check_tensors(k_cache=k_cache, block_table=block_table, from_lens=from_lens, to_lens=to_lens, bounds=bounds)
