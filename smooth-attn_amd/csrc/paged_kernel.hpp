@@ -178,7 +178,9 @@ __global__ __launch_bounds__(256) void paged_plan_kernel(PagedParams p) {
 // fp16 values split exactly).  With a split operand the fp32 weights are
 // split too, and each product becomes the three MFMAs hi*hi + hi*lo + lo*hi:
 // about 2^-16 relative error per product, against the reference's fp32
-// arithmetic (kernels.py:2716-2717, :2746, :2765).
+// arithmetic (kernels.py:2716-2717, :2746, :2765).  Where q and the caches share a
+// 16-bit type the weights are rounded to it for the second product (half a step
+// each), which keeps that to one MFMA; the row sums take them in 32 bits.
 // e4m3fn cache elements (one byte each).  Every e4m3fn value is a bf16
 // value, so fp8 caches widen to bf16 exactly, with no lo part.
 struct fp8e4 {

@@ -157,8 +157,11 @@ struct BoundsParams {
 // negated ones, so both are the same operation: at the last exchange the lower
 // half of the wave takes over the one kind and the upper half the other.  Four
 // prompts of 8192 to 16384 tokens, Hkv 8, D = 128 bf16: 26 us, 4.4 TB/s (37 us with
-// both kinds exchanged over LDS and one page's loads behind another's); e4m3fn
-// keys take 1.7 times their bytes, for unpacking.
+// both kinds exchanged over LDS and one page's loads behind another's); fp32 keys
+// 47 us, 5.2 TB/s.  Where kAhead reads are more rows than a page has, they read and
+// compare its last row again: at pages of 16 half of the rows of e4m3fn keys (22 us,
+// 2.7 TB/s) and of D = 64 bf16 ones (20 us, 3.0 TB/s), three quarters of D = 64
+// e4m3fn ones (22 us, 1.4 TB/s).
 constexpr int kAhead = 4;
 template <typename E, int LPR>
 __global__ __launch_bounds__(256) void paged_bounds_kernel(BoundsParams p) {
@@ -724,7 +727,10 @@ int check_pages(int B, int Hkv, int D, int page_size, int max_pages, int n_pages
     return bt_stride < max_pages ? SA_ERR_BAD_STRIDE : 0;
 }
 
-// Waves for each of `units`: as many as fill 16 waves a CU, at most `most`.
+// Waves for each of `units`: as many as fill 16 waves a CU, at most `most`.  With 8,
+// 16 and 32: bounds of four prompts 31.7, 25.5 and 25.0 us, after a token of each of
+// 64 sequences 2.8, 3.0 and 3.7; scores and choice for those of 512 to 16384 tokens
+// 42.5, 36.3 and 37.4, for 8 of 65536 to 131072 50, 49 and 50.
 int splits_for(int64_t units, int64_t most) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, (256 * 16 + units - 1) / units)));
 }

@@ -4,7 +4,8 @@
 // For a row x of D elements at position t, with the head dim's weight w:
 //   r = 1 / sqrt(mean(x^2) + eps),  n = r x,  z = w n,
 //   y_d = z_d cos - z_{d+D/2} sin,  y_{d+D/2} = z_{d+D/2} cos + z_d sin
-// in fp32, rounded once, to the output's type.  Backward, with g = dL/dy:
+// in fp32, rounded once, to the output's type (the reciprocal root is v_rsq_f32's,
+// at most 3/4 of a step off).  Backward, with g = dL/dy:
 //   dz_d = g_d cos + g_{d+D/2} sin,  dz_{d+D/2} = g_{d+D/2} cos - g_d sin,
 //   dw = sum over rows of dz n,  h = w dz,
 //   dx = r (h - n mean(h n)) = r h - r^3 x mean(h x)
@@ -261,7 +262,9 @@ __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_kernel(NormParams 
 }
 
 // Backward.  A wave keeps dw of its column pair over all its rows; a block adds
-// its waves' in a fixed order into its row of p.partial.
+// its waves' in a fixed order into its row of p.partial.  STREAM: the reads only;
+// with dq and dk written past the caches as well, [4,32/32,4096,128] takes 149 us
+// for 140, fp32 [4,32/32,2048,128] 172 for 162.
 template <typename T, int L, bool STREAM>
 __global__ __launch_bounds__(64 * kBlockWaves) void norm_rope_bwd_kernel(NormParams p) {
     __shared__ float red[kBlockWaves][16 * L];
@@ -403,7 +406,12 @@ int lanes_for(int D) {
 
 // Heads per chunk and the shape of a wave's rows.  heads: the heads of each
 // side; heads_inner: whether a token's heads lie next to each other.  A chunk
-// is halved while the launch has fewer than 16 waves for each CU.
+// is halved while the launch has fewer than 16 waves for each CU.  Forward of
+// [2,32/8,1023,128] bf16 with 4, 8, 16 and 32: 11.3, 9.9, 9.3 and 10.4 us where
+// tokens are neighbours, 9.5, 9.4, 9.3 and 10.5 where heads are; 700 packed tokens
+// 6.5, 6.5, 6.0 and 6.0; long ones the same.  The backward of short launches would
+// rather have 8 ([2,32/8,1023,128] 20.8 -> 16.8 us, [4,12/12,1024,64] 16.8 -> 12.8:
+// a wave's sums of dw cost as much as a row).
 NormGrid plan_norm(const int* heads, int sides, int64_t tokens, int D, bool heads_inner) {
     NormGrid g{};
     g.lanes = lanes_for(D);
@@ -518,7 +526,10 @@ void set_chunks(NormParams& p, const NormGrid& g, const int* heads, int sides) {
 
 // Blocks of the backward's grid along the tokens: about six on each CU in all
 // (the partials that they make are added up in 4 us), each with as many tiles as
-// the others.
+// the others.  With 3, 6 and 12 (sums of the partials included):
+// [4,12/12,1024,64] fp16 13.4, 16.8 and 16.9 us, [2,32/8,1023,128] bf16 16.7, 20.8
+// and 20.8, fp32 24.4, 26.1 and 26.1, [4,32/32,4096,128] bf16 138, 140 and 144,
+// fp32 [4,32/32,2048,128] 163, 162 and 151.
 int64_t bwd_blocks(const NormGrid& g) {
     const int64_t most = std::max<int64_t>(1, kCus * 6 / g.chunks);
     const int64_t rounds = (g.blocks + most - 1) / most;
