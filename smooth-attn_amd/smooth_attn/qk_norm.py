@@ -107,6 +107,7 @@ def _qk_norm_rope_bwd(q, k, gq, gk, q_weight, k_weight, cos, sin, positions, eps
     if (k.shape != (B, Hkv, T, D) or gq.shape != q.shape or gk.shape != k.shape or cos.shape[0] == 0 < B * T
             or (positions is not None and (positions.dtype != torch.int32 or positions.shape not in ((T,), (B, T))))):
         raise ValueError("the saved tensors of the norm must have the shapes and types that forward saved")
+    q, k = _flash_operand(q), _flash_operand(k)
     dq, dk = _output_like(q), _output_like(k)
     dqw = torch.empty_like(q_weight) if need_qw else None
     dkw = torch.empty_like(k_weight) if need_kw else None
@@ -115,7 +116,6 @@ def _qk_norm_rope_bwd(q, k, gq, gk, q_weight, k_weight, cos, sin, positions, eps
     cos, sin = _rope_tables(cos, sin, T, D)
     if positions is not None:
         positions = positions.contiguous()
-    q, k = _flash_operand(q), _flash_operand(k)
     gq, gk = _flash_operand(gq.to(q.dtype)), _flash_operand(gk.to(q.dtype))
     (qw, kw), w_code = _norm_weights(q.dtype, q_weight, k_weight)
     w_dtype = next((w.dtype for w in (qw, kw) if w is not None), q.dtype)
