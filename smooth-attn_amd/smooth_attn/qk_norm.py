@@ -28,6 +28,9 @@ def _check_norm_args(names, tensors, weights, cos, sin, D):
                          f"{'/'.join(str(t.dtype) for t in tensors)}")
     if D % 16 or not 16 <= D <= 512:
         raise ValueError(f"the norm supports head dims that are multiples of 16 in 16..512, got {D}")
+    if any(t.shape[1] > MAX_NORM_HEADS for t in tensors):
+        raise ValueError(f"the norm takes at most {MAX_NORM_HEADS} heads of {'/'.join(names)}, got "
+                         f"{'/'.join(str(t.shape[1]) for t in tensors)}")
     for name, w in zip(("q_weight", "k_weight"), weights):
         if w is not None and (w.shape != (D,) or w.dtype not in (torch.float32, first.dtype)):
             raise ValueError(f"{name} must be [{D}] of {first.dtype} or float32, got {tuple(w.shape)} of {w.dtype}")
@@ -42,6 +45,8 @@ def _check_norm_args(names, tensors, weights, cos, sin, D):
 _INT_DTYPES = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 # Tokens of one launch (heads and head dims past them make up the rest of 2^32 threads).
 MAX_NORM_TOKENS = 1 << 24
+# Heads of q or of k (each may be a row of the launch's grid).
+MAX_NORM_HEADS = 65535 // 4
 
 
 def _int32(name, t):
@@ -160,7 +165,7 @@ def sp2norm_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, 
     pass, with gradients of q, k and both weights.
 
     q: [B, Hq, T, D], k: [B, Hkv, T, D], bf16, fp16 or fp32, D a multiple of 16
-    up to 512, any strides (those of a projection's [B, T, H, D] output are read
+    up to 512, at most 2^24 tokens and 16383 heads, any strides (those of a projection's [B, T, H, D] output are read
     and written as they lie).  q_weight, k_weight: [D] of q's dtype or fp32, or
     None for ones.  cos, sin: [n_pos, D/2] (precompute_rope_cos_sin); row t of
     the tables turns token t, or row positions[t] / positions[b, t] where an
