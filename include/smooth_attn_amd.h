@@ -477,7 +477,8 @@ int sa_paged_kv_append_lens(const void* k_new, const void* v_new,
  * row (b, t) uses table row positions[b * pos_stride + t] (int32; NULL: row
  * t), clamped to the table.  Weights: w_dtype SA_F32 or dtype.  D a multiple
  * of 16 in 16..512; element strides (b, h, t, d) with unit d stride, the
- * others multiples of 16 bytes; pointers 16-byte aligned; B * T <= 2^24.
+ * others multiples of 16 bytes; pointers 16-byte aligned; B * T <= 2^24, Hq and
+ * Hkv <= 16383.
  * No counterpart in the reference.
  */
 int sa_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, void* k_out,

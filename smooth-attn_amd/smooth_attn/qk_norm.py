@@ -165,11 +165,12 @@ def sp2norm_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, positions=None, 
     pass, with gradients of q, k and both weights.
 
     q: [B, Hq, T, D], k: [B, Hkv, T, D], bf16, fp16 or fp32, D a multiple of 16
-    up to 512, at most 2^24 tokens and 16383 heads, any strides (those of a projection's [B, T, H, D] output are read
-    and written as they lie).  q_weight, k_weight: [D] of q's dtype or fp32, or
-    None for ones.  cos, sin: [n_pos, D/2] (precompute_rope_cos_sin); row t of
-    the tables turns token t, or row positions[t] / positions[b, t] where an
-    integer tensor [T] or [B, T] is given (clamped to the tables).
+    up to 512, at most 2^24 tokens and 16383 heads, any strides (those of a
+    projection's [B, T, H, D] output are read and written as they lie).  q_weight,
+    k_weight: [D] of q's dtype or fp32, or None for ones.  cos, sin: [n_pos, D/2]
+    (precompute_rope_cos_sin); row t of the tables turns token t, or row
+    positions[t] / positions[b, t] where an integer tensor [T] or [B, T] is given
+    (clamped to the tables).
 
     ``z = x * rsqrt(mean(x^2) + eps) * weight``, then the pair (d, d + D/2) of z
     is turned by its angle; fp32 inside, rounded once.  Returns (q', k') for
